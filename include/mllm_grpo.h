@@ -323,6 +323,150 @@ int mllm_lm_head_partials(const mllm_lm_head_args* args, void* stream);
 int32_t mllm_lm_head_splits(int64_t n_rows, int64_t vocab);
 int64_t mllm_lm_head_partials_bytes(int64_t n_rows, int64_t vocab);
 
+/* ---- preference loss (paired log ratios), forward and backward ----
+ * Sequences 0..n_pairs-1 are the chosen answers, sequence n_pairs + p is the rejected answer of pair p.  With
+ *   lp_s  = sum_t mask_st * lp_st                (divided by sum_t mask_st with average; 0 for an empty mask)
+ *   d_s   = lp_s - ref_s                         (ref_s reduced like lp_s, or given per sequence; 0 without ref_logps)
+ *   h_p   = d_p - d_(n_pairs + p)
+ *   SIGMOID  l_p = -(1-e) log sigmoid(beta h_p) - e log sigmoid(-beta h_p),  e = label_smoothing
+ *   HINGE    l_p = max(0, 1 - beta h_p)
+ *   IPO      l_p = (h_p - 1/(2 beta))^2
+ *   loss  = sum_p pair_weights_p * l_p / total_pairs
+ * A position whose mask is 0 takes no part: its logits, log-prob and reference log-prob may hold anything.  The
+ * sequence sums, the loss and its derivative are formed in double precision in a fixed order.  The reference has
+ * no preference loss; the operator scores rows exactly as mllm_grpo_fwd does (same geometry, ids, mask, soft-cap). */
+typedef enum mllm_grpo_preference_kind {
+  MLLM_GRPO_PREFERENCE_SIGMOID = 0,
+  MLLM_GRPO_PREFERENCE_HINGE = 1,
+  MLLM_GRPO_PREFERENCE_IPO = 2
+} mllm_grpo_preference_kind;
+
+typedef struct mllm_grpo_preference_args {
+  uint64_t struct_size;  /* sizeof(mllm_grpo_preference_args) */
+  int64_t n_pairs;       /* P > 0; there are 2P sequences */
+  int64_t seq_rows;      /* L >= scored_rows */
+  int64_t scored_rows;   /* T > 0 */
+  int64_t vocab;
+  int64_t row_stride;    /* elements between rows of logits AND dlogits, >= vocab */
+  int32_t kind;          /* mllm_grpo_preference_kind */
+  int32_t average;       /* 1: log-probs averaged over the valid tokens of a sequence instead of summed */
+  float beta;            /* > 0 */
+  float label_smoothing; /* [0, 0.5], SIGMOID only */
+  float softcap;         /* 0 = off */
+  float grad_scale;      /* cotangent of the loss, used when grad_scale_dev is NULL */
+  float total_pairs;     /* > 0; normaliser, used when total_pairs_dev is NULL */
+  int32_t ref_per_sequence; /* 0: ref_logps is [2P*T]; 1: [2P], the reference's lp_s */
+  const void* logits;       /* bf16 [2P, seq_rows, row_stride] */
+  const int32_t* chosen_ids;   /* [2P*T] */
+  const float* token_logps;    /* [2P*T], mllm_grpo_preference_logps only */
+  const float* mask;           /* [2P*T] weights, or NULL = every scored row counts */
+  const float* ref_logps;      /* or NULL */
+  const float* pair_weights;   /* [P] or NULL */
+  const float* total_pairs_dev;/* scalar in device memory or NULL */
+  const float* grad_scale_dev; /* scalar in device memory or NULL */
+  float* loss;             /* [1] */
+  float* rewards;          /* [2P] beta * d_s */
+  float* sequence_logps;   /* [2P] lp_s, or NULL */
+  float* dtoken_logps;     /* [2P*T] d loss / d token_logps, mllm_grpo_preference_logps only; or NULL */
+  void* dlogits;           /* bf16, may alias logits */
+  void* workspace;         /* mllm_grpo_preference_workspace_bytes(...), 16-byte aligned; carries the residuals from
+                              mllm_grpo_preference_fwd to mllm_grpo_preference_bwd */
+  int32_t* device_status;  /* optional */
+} mllm_grpo_preference_args;
+
+/* Forward from logits: loss, rewards, sequence_logps and the residuals of the backward.  Rows with mask 0 are not read. */
+int mllm_grpo_preference_fwd(const mllm_grpo_preference_args* args, void* stream);
+/* Backward: dlogits of every row (zeros where the mask is 0 and in rows >= scored_rows) from the residuals. */
+int mllm_grpo_preference_bwd(const mllm_grpo_preference_args* args, void* stream);
+/* Both (grad_scale known up front). */
+int mllm_grpo_preference_fwd_bwd(const mllm_grpo_preference_args* args, void* stream);
+/* The same loss from per-token log-probs (those of mllm_lm_head_partials + mllm_grpo_combine, for instance) with
+ * its gradient with respect to them. */
+int mllm_grpo_preference_logps(const mllm_grpo_preference_args* args, void* stream);
+int64_t mllm_grpo_preference_workspace_bytes(int64_t n_pairs, int64_t scored_rows);
+
+/* ---- embedding table: scaled lookup and its gradient ----
+ * out[n, :] = scale * weight[ids[n] - vocab_start, :], the product in f32, rounded once to the table's type.
+ * Ids outside [vocab_start, vocab_start + vocab) but inside [0, vocab_total) belong to another vocabulary shard
+ * and give a zero row (the shards' outputs add up); ids outside [0, vocab_total) give a zero row, get no gradient
+ * and raise MLLM_GRPO_DEV_ID_IGNORED. */
+#define MLLM_GRPO_DEV_ID_IGNORED 4
+typedef enum mllm_grpo_dtype { MLLM_GRPO_BF16 = 0, MLLM_GRPO_F16 = 1, MLLM_GRPO_F32 = 2 } mllm_grpo_dtype;
+
+typedef struct mllm_grpo_embedding_args {
+  uint64_t struct_size;  /* sizeof(mllm_grpo_embedding_args) */
+  int64_t n_tokens;      /* >= 0; with 0 the lookup does nothing and the gradient is all zeros */
+  int64_t vocab;         /* rows of the table held by this call */
+  int64_t hidden;        /* H */
+  int64_t weight_stride; /* elements between rows of weight (lookup) or of dweight (gradient), >= hidden */
+  int64_t token_stride;  /* elements between rows of out (lookup) or of grad_out (gradient), >= hidden */
+  int64_t vocab_start;
+  int64_t vocab_total;   /* 0 means vocab_start + vocab */
+  float scale;
+  int32_t dtype;         /* mllm_grpo_dtype of weight and out (lookup), of grad_out (gradient) */
+  int32_t out_dtype;     /* of dweight (gradient) */
+  int32_t accumulate;    /* gradient: 1 adds to dweight (f32 only; rows without tokens are not touched), 0 writes all of it */
+  const int32_t* ids;    /* [n_tokens] */
+  const void* weight;    /* lookup */
+  void* out;             /* lookup */
+  const void* grad_out;  /* gradient */
+  void* dweight;         /* gradient */
+  void* workspace;       /* gradient: mllm_grpo_embedding_workspace_bytes(...), 16-byte aligned */
+  int32_t* device_status;/* optional */
+} mllm_grpo_embedding_args;
+int mllm_grpo_embedding_lookup(const mllm_grpo_embedding_args* args, void* stream);
+/* dweight[v, :] = scale * sum over n with ids[n] == v of grad_out[n, :]: the tokens are sorted by id first (stable,
+ * one launch), so every row is summed in f32 in an order that depends on the ids alone; no floating-point atomics. */
+int mllm_grpo_embedding_grad(const mllm_grpo_embedding_args* args, void* stream);
+int64_t mllm_grpo_embedding_workspace_bytes(int64_t n_tokens, int64_t hidden);
+
+/* ---- 8-bit floating point (e4m3) with a scale for each block of 128 ----
+ * scale = max(amax, 448 * 2^-126) / 448 over a block of block_rows x 128 elements, q = e4m3(448 x / amax) to nearest
+ * even; blocks at the right and lower edge are shorter.  A NaN stays a NaN and is left out of the maximum; an
+ * infinity makes its block's scale infinite. */
+typedef struct mllm_lm_head_fp8_quantize_args {
+  uint64_t struct_size;
+  int64_t rows, cols;     /* >= 0, > 0 */
+  int64_t x_stride;       /* elements between rows of x, >= cols */
+  int64_t q_stride;       /* bytes between rows of q, >= cols */
+  int32_t block_rows;     /* 1 (activations) or 128 (weights) */
+  int32_t dtype;          /* mllm_grpo_dtype of x */
+  const void* x;
+  void* q;                /* e4m3 [rows, cols] */
+  float* scales;          /* [ceil(rows / block_rows), ceil(cols / 128)] */
+} mllm_lm_head_fp8_quantize_args;
+int mllm_lm_head_fp8_quantize(const mllm_lm_head_fp8_quantize_args* args, void* stream);
+
+/* y[m, n] = sum_b x_scales[m, b] * w_scales[n / 128, b] * sum_{k in block b} x[m, k] * w[n, k] on the tensor cores,
+ * inner sums, block products and the sum over blocks in f32, rounded once to out_dtype. */
+typedef struct mllm_lm_head_fp8_args {
+  uint64_t struct_size;
+  int64_t n_rows;         /* M; >= 0 for the product, > 0 for the partials */
+  int64_t vocab;          /* N > 0 */
+  int64_t hidden_dim;     /* K > 0, a multiple of 16 */
+  int64_t hidden_stride;  /* bytes between rows of hidden, >= hidden_dim, a multiple of 16 */
+  int64_t weight_stride;  /* bytes between rows of weight, likewise */
+  int64_t out_stride;     /* elements between rows of out, >= vocab (product) */
+  int64_t vocab_start, vocab_total; /* partials: as in mllm_lm_head_args */
+  float softcap;          /* partials */
+  int32_t reserved;       /* 0 */
+  int32_t out_dtype;      /* product: MLLM_GRPO_BF16, _F16 or _F32 */
+  const void* hidden;         /* e4m3 [M, K], 16-byte aligned */
+  const float* hidden_scales; /* [M, ceil(K / 128)] */
+  const void* weight;         /* e4m3 [N, K], 16-byte aligned */
+  const float* weight_scales; /* [ceil(N / 128), ceil(K / 128)] */
+  void* out;                  /* product */
+  const int32_t* chosen_ids;  /* partials: [M] */
+  void* partials;             /* partials: mllm_lm_head_fp8_partials_bytes(n_rows, vocab) bytes, 16-byte aligned */
+  int32_t* device_status;     /* optional */
+} mllm_lm_head_fp8_args;
+int mllm_lm_head_fp8_matmul(const mllm_lm_head_fp8_args* args, void* stream);
+/* mllm_lm_head_partials with both operands in 8 bits.  The first n_rows records of `partials` are the rows' merged
+ * (max, sumexp, sum e*y, chosen-or-0), to go through mllm_grpo_combine with n_shards = 1 (or, all-gathered over a
+ * sharded head's ranks, n_shards = ranks); the rest of the buffer is scratch. */
+int mllm_lm_head_fp8_partials(const mllm_lm_head_fp8_args* args, void* stream);
+int64_t mllm_lm_head_fp8_partials_bytes(int64_t n_rows, int64_t vocab);
+
 /* Bytes of loss_terms scratch a problem of n_tokens = B*T needs. */
 int64_t mllm_grpo_workspace_bytes(int64_t n_tokens);
 

@@ -15,6 +15,8 @@ FLAG_CE_LOSS = 2
 LM_HEAD_FLAG_WEIGHT_HV = 256
 DEV_ID_CLAMPED = 1
 DEV_WAIT_TIMEOUT = 2
+DEV_ID_IGNORED = 4
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
 
 EXPORTS = (
     "mllm_grpo_fwd", "mllm_grpo_bwd", "mllm_grpo_fwd_bwd", "mllm_grpo_fwd_partials", "mllm_grpo_combine",
@@ -23,6 +25,11 @@ EXPORTS = (
     "mllm_grpo_fwd_bwd_sharded", "mllm_grpo_exchange_bytes", "mllm_grpo_set_plan_override",
     "mllm_grpo_entropy_stats", "mllm_grpo_scale_grad", "mllm_ppo_value_loss", "mllm_ppo_value_workspace_bytes",
     "mllm_lm_head_partials", "mllm_lm_head_splits", "mllm_lm_head_partials_bytes", "mllm_grpo_partial_width",
+    "mllm_grpo_preference_fwd", "mllm_grpo_preference_bwd", "mllm_grpo_preference_fwd_bwd",
+    "mllm_grpo_preference_logps", "mllm_grpo_preference_workspace_bytes",
+    "mllm_grpo_embedding_lookup", "mllm_grpo_embedding_grad", "mllm_grpo_embedding_workspace_bytes",
+    "mllm_lm_head_fp8_quantize", "mllm_lm_head_fp8_matmul", "mllm_lm_head_fp8_partials",
+    "mllm_lm_head_fp8_partials_bytes",
 )
 
 
@@ -77,6 +84,60 @@ class LmHeadArgs(C.Structure):
     ]
 
 
+class PreferenceArgs(C.Structure):
+    """Mirror of `struct mllm_grpo_preference_args`."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint64),
+        ("n_pairs", C.c_int64), ("seq_rows", C.c_int64), ("scored_rows", C.c_int64), ("vocab", C.c_int64),
+        ("row_stride", C.c_int64), ("kind", C.c_int32), ("average", C.c_int32), ("beta", C.c_float),
+        ("label_smoothing", C.c_float), ("softcap", C.c_float), ("grad_scale", C.c_float), ("total_pairs", C.c_float),
+        ("ref_per_sequence", C.c_int32),
+        ("logits", C.c_void_p), ("chosen_ids", C.c_void_p), ("token_logps", C.c_void_p), ("mask", C.c_void_p),
+        ("ref_logps", C.c_void_p), ("pair_weights", C.c_void_p), ("total_pairs_dev", C.c_void_p),
+        ("grad_scale_dev", C.c_void_p), ("loss", C.c_void_p), ("rewards", C.c_void_p), ("sequence_logps", C.c_void_p),
+        ("dtoken_logps", C.c_void_p), ("dlogits", C.c_void_p), ("workspace", C.c_void_p),
+        ("device_status", C.c_void_p),
+    ]
+
+
+class EmbeddingArgs(C.Structure):
+    """Mirror of `struct mllm_grpo_embedding_args`."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint64),
+        ("n_tokens", C.c_int64), ("vocab", C.c_int64), ("hidden", C.c_int64), ("weight_stride", C.c_int64),
+        ("token_stride", C.c_int64), ("vocab_start", C.c_int64), ("vocab_total", C.c_int64),
+        ("scale", C.c_float), ("dtype", C.c_int32), ("out_dtype", C.c_int32), ("accumulate", C.c_int32),
+        ("ids", C.c_void_p), ("weight", C.c_void_p), ("out", C.c_void_p), ("grad_out", C.c_void_p),
+        ("dweight", C.c_void_p), ("workspace", C.c_void_p), ("device_status", C.c_void_p),
+    ]
+
+
+class Fp8QuantizeArgs(C.Structure):
+    """Mirror of `struct mllm_lm_head_fp8_quantize_args`."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint64),
+        ("rows", C.c_int64), ("cols", C.c_int64), ("x_stride", C.c_int64), ("q_stride", C.c_int64),
+        ("block_rows", C.c_int32), ("dtype", C.c_int32),
+        ("x", C.c_void_p), ("q", C.c_void_p), ("scales", C.c_void_p),
+    ]
+
+
+class Fp8Args(C.Structure):
+    """Mirror of `struct mllm_lm_head_fp8_args`."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint64),
+        ("n_rows", C.c_int64), ("vocab", C.c_int64), ("hidden_dim", C.c_int64), ("hidden_stride", C.c_int64),
+        ("weight_stride", C.c_int64), ("out_stride", C.c_int64), ("vocab_start", C.c_int64),
+        ("vocab_total", C.c_int64), ("softcap", C.c_float), ("reserved", C.c_int32), ("out_dtype", C.c_int32),
+        ("hidden", C.c_void_p), ("hidden_scales", C.c_void_p), ("weight", C.c_void_p), ("weight_scales", C.c_void_p),
+        ("out", C.c_void_p), ("chosen_ids", C.c_void_p), ("partials", C.c_void_p), ("device_status", C.c_void_p),
+    ]
+
+
 class GrpoError(RuntimeError):
     def __init__(self, fn: str, status: int, text: str, cuda: str = ""):
         self.status = status
@@ -114,6 +175,19 @@ def load():
     lib.mllm_lm_head_splits.restype = C.c_int32
     lib.mllm_lm_head_partials_bytes.argtypes = [C.c_int64, C.c_int64]
     lib.mllm_lm_head_partials_bytes.restype = C.c_int64
+    for name, args in (("mllm_grpo_preference_fwd", PreferenceArgs), ("mllm_grpo_preference_bwd", PreferenceArgs),
+                       ("mllm_grpo_preference_fwd_bwd", PreferenceArgs), ("mllm_grpo_preference_logps", PreferenceArgs),
+                       ("mllm_grpo_embedding_lookup", EmbeddingArgs), ("mllm_grpo_embedding_grad", EmbeddingArgs),
+                       ("mllm_lm_head_fp8_quantize", Fp8QuantizeArgs), ("mllm_lm_head_fp8_matmul", Fp8Args),
+                       ("mllm_lm_head_fp8_partials", Fp8Args)):
+        fn = getattr(lib, name)
+        fn.argtypes = [C.POINTER(args), C.c_void_p]
+        fn.restype = C.c_int
+    for name in ("mllm_grpo_preference_workspace_bytes", "mllm_grpo_embedding_workspace_bytes",
+                 "mllm_lm_head_fp8_partials_bytes"):
+        fn = getattr(lib, name)
+        fn.argtypes = [C.c_int64, C.c_int64]
+        fn.restype = C.c_int64
     lib.mllm_ppo_value_workspace_bytes.argtypes = [C.c_int64, C.c_int64]
     lib.mllm_ppo_value_workspace_bytes.restype = C.c_int64
     lib.mllm_grpo_workspace_bytes.argtypes = [C.c_int64]

@@ -1,0 +1,26 @@
+// What the kernels of the block-scaled 8-bit product share.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace grpo {
+namespace fp8 {
+
+struct Params {
+  int64_t n_rows, vocab, hidden, hidden_stride, weight_stride, out_stride, vocab_start, vocab_total;
+  int m_tiles, n_tiles, k_blocks, tiles_per_split, splits;
+  int out_aligned;  // rows of out start on 16-byte boundaries
+  float softcap;
+  const uint8_t* x;
+  const uint8_t* w;
+  const float* x_scales;
+  const float* w_scales;
+  void* out;
+  const int32_t* chosen_ids;
+  float4* partials;  // [1 + ranges, n_rows]: the merged entry, then one entry per column range
+  int32_t* device_status;
+};
+
+}  // namespace fp8
+}  // namespace grpo

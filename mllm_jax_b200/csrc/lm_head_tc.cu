@@ -17,16 +17,13 @@
 //               fills the other accumulator
 // Every mbarrier wait is bounded by wall-clock time; a wait that runs out raises a status bit, makes all
 // roles leave their loops, and the CTA still frees its tensor memory before it returns.
-#include <cuda.h>
-
-#include <mutex>
-
-#include "grpo_cluster.cuh"
-#include "grpo_common.cuh"
 #include "grpo_launch.h"
+#include "grpo_tc.cuh"
 
 namespace grpo {
 namespace lmh {
+
+using namespace tc;
 
 constexpr int kBM = 128;      // rows per CTA tile (TMEM lanes)
 constexpr int kBN = 256;      // vocabulary columns per tile (one accumulator)
@@ -37,7 +34,6 @@ constexpr int kBBytes = kBN * kBK * 2;  // 32 KB
 constexpr int kStageBytes = kABytes + kBBytes;
 constexpr int kThreads = 192;
 constexpr int kTmemCols = 512;
-constexpr unsigned long long kWaitNs = 2000000000ull;  // 2 s per wait
 constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + 1024 /* alignment slack */ + 256 /* barriers */;
 
 struct Params {
@@ -50,28 +46,6 @@ struct Params {
   int32_t* device_status;
 };
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
-      : "memory");
-}
-__device__ __forceinline__ void prefetch_tmap(const CUtensorMap* map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
-}
-
-// Shared-memory matrix descriptor of a K-major bf16 tile whose rows are 128 bytes (64 elements), stored
-// with the 128-byte swizzle in groups of 8 rows (1024 bytes): start address and stride between row groups
-// in units of 16 bytes, descriptor version 1, layout type 2 (128-byte swizzle).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
-  uint64_t d = 0;
-  d |= uint64_t((addr & 0x3FFFFu) >> 4);
-  d |= uint64_t(1) << 16;            // leading byte offset: unused for swizzled K-major tiles
-  d |= uint64_t(1024 >> 4) << 32;    // stride byte offset: next group of 8 rows
-  d |= uint64_t(1) << 46;            // descriptor version
-  d |= uint64_t(2) << 61;            // 128-byte swizzle
-  return d;
-}
 // The same for an MN-major operand (the weight stored [hidden, vocab], vocabulary contiguous): 64 vocabulary
 // entries (128 bytes) per row of the swizzle atom, 8 k-rows per atom (1024 bytes, the stride offset), and the
 // leading offset is the distance between two 64-entry column blocks of the tile.
@@ -97,44 +71,6 @@ __device__ __forceinline__ void mma_bf16(uint32_t tmem_d, uint64_t adesc, uint64
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// Bounded mbarrier wait shared by the three roles: false once any wait of the CTA has run out.
-__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
-  if (cl::mbar_try(bar, parity)) return true;
-  unsigned long long t0 = 0;
-  for (uint32_t spin = 0;; ++spin) {
-    if (cl::mbar_try(bar, parity)) return true;
-    if (*abort_flag) return false;
-    if ((spin & 255u) == 0) {
-      const unsigned long long now = cl::globaltimer();
-      if (t0 == 0) t0 = now;
-      if (now - t0 > kWaitNs) {
-        *abort_flag = 1;
-        if (status) atomicOr(status, MLLM_GRPO_DEV_WAIT_TIMEOUT);
-        return false;
-      }
-    }
-  }
-}
-
 // WMN: the weight is [hidden, vocab] (vocabulary contiguous, a flax Dense kernel) instead of [vocab, hidden].
 template <bool WMN>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -354,26 +290,6 @@ lm_head_stats_kernel(const __grid_constant__ CUtensorMap map_hidden, const __gri
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(uint32_t(kTmemCols)) : "memory");
   }
-}
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no link-time dependency on libcuda).
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static std::once_flag once;
-  static EncodeTiledFn fn = nullptr;
-  std::call_once(once, [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-    else
-      (void)cudaGetLastError();
-  });
-  return fn;
 }
 
 // bf16 [rows, cols] row-major with `ld` elements between rows -> tiles of box_rows x 64 columns, 128-byte swizzle.

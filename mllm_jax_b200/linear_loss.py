@@ -18,15 +18,16 @@ loss value itself) never write or read a logits tensor at all.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
 from . import _lib
+from .fp8 import Fp8Blocks, _bind, quantize_fp8
 from .ops import LossConfig, TokenLossProblem
 
 
-def lm_head_forward(hidden: torch.Tensor, weight: torch.Tensor, token_ids: torch.Tensor,
+def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks], token_ids: torch.Tensor,
                     mask: Optional[torch.Tensor] = None, advantages: Optional[torch.Tensor] = None,
                     total_valid_token_count=None, old_per_token_logps: Optional[torch.Tensor] = None,
                     ref_per_token_logps: Optional[torch.Tensor] = None, *, cfg: Optional[LossConfig] = None,
@@ -46,21 +47,32 @@ def lm_head_forward(hidden: torch.Tensor, weight: torch.Tensor, token_ids: torch
     (the reference-model pass, train_modules/__init__.py:129-132, and plugins/training/update/ppo.py:39-43).
     Two launches: the tensor-core kernel writes per-row partials for each vocabulary range, and
     mllm_grpo_combine merges them and runs the per-token epilogue.  H must be a multiple of 64.
-    The logits are the f32 accumulators (not rounded to bf16 on the way)."""
+    The logits are the f32 accumulators (not rounded to bf16 on the way).
+
+    weight may be `Fp8Blocks` [V, H] with blocks of (128, 128) (`quantize_fp8(weight, block=(128, 128))`): hidden is
+    quantised with a scale per 1 x 128 on the way in and both run as 8-bit operands (mllm_lm_head_fp8_partials; H a
+    multiple of 16, any distance between the rows of hidden).  The head of a frozen reference model takes half the
+    memory that way; the log-probs are those of the quantised operands."""
     cfg = cfg or LossConfig()
+    fp8 = isinstance(weight, Fp8Blocks)
     if hidden.dim() == 2:
         hidden = hidden.unsqueeze(0)
         token_ids = token_ids.reshape(1, -1)
     if not hidden.is_cuda:
         raise RuntimeError("lm_head_forward needs CUDA tensors: the kernels have no CPU path")
-    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+    if hidden.dtype != torch.bfloat16 or (not fp8 and weight.dtype != torch.bfloat16):
         raise TypeError("hidden and weight must be bfloat16")
     B, T, H = hidden.shape
+    if fp8 and weight_layout != "vh":
+        raise ValueError("an 8-bit weight is [V, H]")
     if weight_layout not in ("vh", "hv"):
         raise ValueError("weight_layout must be 'vh' ([V, H]) or 'hv' ([H, V])")
     hv = weight_layout == "hv"
     V = weight.shape[1] if hv else weight.shape[0]
-    if weight.shape[0 if hv else 1] != H or hidden.stride(2) != 1 or weight.stride(1) != 1 or \
+    if fp8:
+        if weight.shape[1] != H:
+            raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not match")
+    elif weight.shape[0 if hv else 1] != H or hidden.stride(2) != 1 or weight.stride(1) != 1 or \
             hidden.stride(0) != T * hidden.stride(1):
         raise ValueError(f"hidden {tuple(hidden.shape)} / weight {tuple(weight.shape)}: need [B, T, H] rows evenly "
                          "spaced and a [V, H] (or [H, V]) weight with unit stride along its last dimension")
@@ -69,8 +81,15 @@ def lm_head_forward(hidden: torch.Tensor, weight: torch.Tensor, token_ids: torch
     dev = hidden.device
     N = B * T
     lib = _lib.load()
-    splits = int(lib.mllm_lm_head_splits(N, V))
-    nbytes = int(lib.mllm_lm_head_partials_bytes(N, V))
+    if fp8:
+        with torch.cuda.device(dev):
+            hq = quantize_fp8(hidden.reshape(N, H), block=(1, 128))
+        a = _bind(hq, weight)
+        splits, nbytes = 1, int(lib.mllm_lm_head_fp8_partials_bytes(N, V))
+    else:
+        a = _lib.LmHeadArgs()
+        splits = int(lib.mllm_lm_head_splits(N, V))
+        nbytes = int(lib.mllm_lm_head_partials_bytes(N, V))
     if workspace is None:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     elif workspace.numel() * workspace.element_size() < nbytes or workspace.data_ptr() % 16:
@@ -83,30 +102,32 @@ def lm_head_forward(hidden: torch.Tensor, weight: torch.Tensor, token_ids: torch
     v_all = int(vocab_total) if vocab_total is not None else int(vocab_start) + V
     TokenLossProblem._init_side(prob, B, T, T, v_all, dev, token_ids, mask, advantages, total_valid_token_count,
                                 old_per_token_logps, ref_per_token_logps, cfg)
-    a = _lib.LmHeadArgs()
-    a.n_rows, a.vocab, a.hidden_dim = N, V, H
-    a.hidden_stride, a.weight_stride = hidden.stride(1), weight.stride(0)
+    if not fp8:
+        a.n_rows, a.vocab, a.hidden_dim = N, V, H
+        a.hidden_stride, a.weight_stride = hidden.stride(1), weight.stride(0)
+        a.flags = (0 if cfg.compute_entropy else _lib.FLAG_SKIP_ENTROPY) | (_lib.LM_HEAD_FLAG_WEIGHT_HV if hv else 0)
+        a.hidden, a.weight = hidden.data_ptr(), weight.data_ptr()
     a.vocab_start, a.vocab_total = int(vocab_start), int(vocab_total) if vocab_total is not None else int(vocab_start) + V
     a.softcap = float(cfg.softcap) if cfg.softcap else 0.0
-    a.flags = (0 if cfg.compute_entropy else _lib.FLAG_SKIP_ENTROPY) | (_lib.LM_HEAD_FLAG_WEIGHT_HV if hv else 0)
-    a.hidden, a.weight = hidden.data_ptr(), weight.data_ptr()
     a.chosen_ids, a.partials = prob.chosen_ids.data_ptr(), workspace.data_ptr()
     a.device_status = prob.device_status.data_ptr()
     with torch.cuda.device(dev):
-        _lib.call("mllm_lm_head_partials", a, torch.cuda.current_stream().cuda_stream)
+        _lib.call("mllm_lm_head_fp8_partials" if fp8 else "mllm_lm_head_partials", a, torch.cuda.current_stream().cuda_stream)
         parts, n_parts = workspace, splits
         if group is not None:
             import torch.distributed as dist
 
             k = dist.get_world_size(group)
-            mine = workspace[:nbytes]
-            parts = torch.empty(k * nbytes, dtype=torch.uint8, device=dev)
+            # the merged records come first in the 8-bit form's buffer, the splits' records are the whole of the other
+            nsend = 16 * N if fp8 else nbytes
+            mine = workspace[:nsend]
+            parts = torch.empty(k * nsend, dtype=torch.uint8, device=dev)
             dist.all_gather_into_tensor(parts, mine, group=group)  # [k, splits, N, 4] f32: rank-major vocabulary ranges
             n_parts = k * splits
         g = prob.args()
         g.gathered_partials, g.n_shards = parts.data_ptr(), n_parts
         _lib.call("mllm_grpo_combine", g, torch.cuda.current_stream().cuda_stream)
-    prob._keepalive = (hidden, weight, workspace, parts)
+    prob._keepalive = (hidden, hq if fp8 else None, weight, workspace, parts)
     out = {"per_token_logps": prob.per_token_logps, "token_entropy": prob.token_entropy, "lse": prob.lse.view(B, T),
            "problem": prob, "splits": splits}
     if not forward_only:

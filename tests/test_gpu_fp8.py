@@ -1,0 +1,243 @@
+"""Block-scaled e4m3: quantising, the product, and the lm_head folded into the loss statistics, against 64-bit forms."""
+import pytest
+import torch
+
+import mllm_jax_b200 as G
+from mllm_jax_b200.linear_loss import lm_head_forward
+from tests import operator_reference as R
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _x(r, c, dtype, seed, dev, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(r, c, generator=g) * torch.exp(spread * torch.randn(r, 1, generator=g))).to(dtype).to(dev)
+
+
+def _check_quantized(q, x, block):
+    values, scales, y = R.quantize(x, block[0])
+    assert torch.equal(q.scales, scales.to(q.scales.device))
+    got = q.values.double()
+    if x.dtype == torch.float32:
+        # a quotient within 2^-19 of a border may fall to either side: half a step and that much more
+        a = y.abs().clamp(2.0 ** -6, 448)
+        half = torch.exp2(torch.floor(torch.log2(a)) - 4)
+        R.assert_within(got, y, half + 2.0 ** -18 * y.abs(), "values")
+    else:
+        assert torch.equal(torch.isnan(got), torch.isnan(values))
+        fine = ~torch.isnan(values)
+        assert torch.equal(got[fine], values[fine])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("block", [(1, 128), (128, 128)])
+@pytest.mark.parametrize("r,c", [(1, 1), (1, 128), (3, 127), (129, 130), (128, 256), (37, 1000), (300, 515), (257, 2048), (5, 16)])
+def test_quantize(cuda, dtype, block, r, c):
+    x = _x(r, c, dtype, r * 1000 + c, cuda)
+    q = G.quantize_fp8(x, block=block)
+    assert q.values.shape == (r, c) and q.values.dtype == torch.float8_e4m3fn
+    _check_quantized(q, x, block)
+
+
+def test_quantize_borders(cuda):
+    """Quotients that are exactly the middle between two e4m3 values go to the even one, whatever the block's maximum."""
+    for dtype in (torch.bfloat16, torch.float16):
+        tops = torch.arange(129, 256, dtype=torch.float32)            # 8-bit maxima
+        x = torch.zeros(tops.numel(), 128)
+        x[:, 0] = tops
+        x[:, 1:] = torch.arange(1, 128, dtype=torch.float32) * 2      # and all even numbers below
+        x = x.to(dtype).to(cuda)
+        assert (x.float().amax(1) <= 255).all()
+        _check_quantized(G.quantize_fp8(x), x, (1, 128))
+        _check_quantized(G.quantize_fp8(-x * 2.0 ** -9), -x * 2.0 ** -9, (1, 128))
+
+
+@pytest.mark.parametrize("block", [(1, 128), (128, 128)])
+def test_quantize_special_values(cuda, block):
+    x = _x(130, 300, torch.bfloat16, 3, cuda)
+    x[0] = 0                                        # a zero row; with tall blocks just small values
+    x[1] *= 1e-38                                   # subnormal results
+    x[2, :128] = 3e38
+    x[5, 7] = float("nan")
+    q = G.quantize_fp8(x, block=block)
+    _check_quantized(q, x, block)
+    z = torch.zeros(130, 300, device=cuda)
+    q = G.quantize_fp8(z, block=block)
+    assert not q.values.float().any() and (q.scales == 2.0 ** -126).all()
+    x[9, 200] = float("-inf")
+    q = G.quantize_fp8(x, block=block)
+    assert torch.isinf(q.scales[9 if block[0] == 1 else 0, 1]) and torch.isnan(q.dequantize()[9, 200])
+
+
+def test_quantize_strides_and_offsets(cuda):
+    for shift, ld in ((0, 400), (1, 401), (2, 404), (4, 408)):
+        big = torch.full((50 * ld + 8,), float("nan"), dtype=torch.bfloat16, device=cuda)
+        view = big[shift:shift + 50 * ld].view(50, ld)[:, :264]
+        view.copy_(_x(50, 264, torch.bfloat16, 5, cuda))
+        for block in ((1, 128), (128, 128)):
+            _check_quantized(G.quantize_fp8(view, block=block), view, block)
+    t = _x(64, 96, torch.float32, 6, cuda).t()     # not row-major: laid out first
+    _check_quantized(G.quantize_fp8(t), t, (1, 128))
+    assert G.quantize_fp8(torch.empty(0, 40, device=cuda)).values.shape == (0, 40)
+
+
+def _operands(M, N, K, seed, dev):
+    x = _x(M, K, torch.bfloat16, seed, dev, 0.5)
+    w = _x(N, K, torch.bfloat16, seed + 1, dev, 0.5) * (K ** -0.5)
+    return G.quantize_fp8(x), G.quantize_fp8(w, block=(128, 128))
+
+
+SHAPES = [
+    (1, 1, 16), (1, 128, 128), (1, 1000, 896), (2, 4099, 272), (7, 300, 3584), (8, 129, 64), (9, 640, 1040), (16, 2048, 512),
+    (17, 257, 384), (33, 513, 160), (64, 1024, 2048), (128, 256, 128), (129, 255, 144), (300, 1111, 400), (257, 4096, 1792),
+    (1000, 20000, 256),
+]
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("out", TYPES)
+def test_matmul(cuda, M, N, K, out):
+    x, w = _operands(M, N, K, M + N + K, cuda)
+    y = G.fp8_matmul(x, w, out_dtype=out)
+    assert y.shape == (M, N) and y.dtype == out
+    ref, mag = R.product(x.values, x.scales, w.values, w.scales)
+    R.assert_within(y, ref, R.product_bound(ref, mag, K) + ref.abs() * R.HALF_STEP[out] + R.TINY_STEP[out], f"{M}x{N}x{K}")
+    assert torch.equal(y, G.fp8_matmul(x, w, out_dtype=out))
+
+
+@pytest.mark.parametrize("M", [1, 12, 200])
+def test_matmul_views(cuda, M):
+    """Operands that are rows of wider buffers, an output with guards around its rows, a tensor quantised on the way."""
+    N, K, ld = 333, 208, 256
+    x, w = _operands(M, N, K, 77, cuda)
+    wide = lambda t, r: torch.full((r, ld), 0x7F, dtype=torch.uint8, device=cuda).view(torch.float8_e4m3fn)  # noqa: E731  (NaNs)
+    bx, bw = wide(x, M), wide(w, N)
+    bx[:, :K].copy_(x.values)
+    bw[:, :K].copy_(w.values)
+    want = G.fp8_matmul(x, w, out_dtype=torch.float32)
+    got = G.fp8_matmul(G.Fp8Blocks(bx[:, :K], x.scales, (1, 128)), G.Fp8Blocks(bw[:, :K], w.scales), out_dtype=torch.float32)
+    assert torch.equal(got, want)
+    for dtype, off, pad in ((torch.bfloat16, 1, 3), (torch.float32, 0, 0), (torch.float32, 4, 11)):
+        buf = torch.full((M * (N + pad) + off + 8,), 7.0, dtype=dtype, device=cuda)
+        view = buf[off:off + M * (N + pad)].view(M, N + pad)[:, :N]
+        assert G.fp8_matmul(x, w, out=view) is view
+        assert torch.equal(view, want.to(dtype))
+        assert (buf[:off] == 7).all() and (buf[off:off + M * (N + pad)].view(M, -1)[:, N:] == 7).all() and (buf[-8:] == 7).all()
+    raw = _x(M, K, torch.bfloat16, 77, cuda, 0.5)
+    assert torch.equal(G.fp8_matmul(raw, w, out_dtype=torch.float32), want)
+    assert G.fp8_matmul(G.quantize_fp8(raw[:0]), w).shape == (0, N)
+
+
+@pytest.mark.parametrize("M", [3, 150])
+def test_matmul_non_finite(cuda, M):
+    """A NaN or an infinite block reaches its own row or its own columns and no others."""
+    N, K = 300, 256
+    x, w = _operands(M, N, K, 80, cuda)
+    ref, mag = R.product(x.values, x.scales, w.values, w.scales)
+    x.values[1, 5] = float("nan")
+    w.scales[1, 0] = float("inf")
+    y = G.fp8_matmul(x, w, out_dtype=torch.float32).double()
+    assert torch.isnan(y[1]).all() and not torch.isfinite(y[:, 128:256]).any()
+    rows = [m for m in range(M) if m != 1]
+    for cols in (slice(0, 128), slice(256, 300)):
+        R.assert_within(y[rows][:, cols], ref[rows][:, cols], R.product_bound(ref, mag, K)[rows][:, cols] + 2.0 ** -24 * ref[rows][:, cols].abs())
+
+
+HEADS = [(1, 1, 64, 256, None), (1, 5, 16, 7, None), (2, 75, 192, 1000, None), (1, 130, 128, 10240, None), (3, 50, 896, 4099, None),
+         (1, 300, 80, 2500, 30.0)]
+
+
+@pytest.mark.parametrize("B,T,H,V,cap", HEADS)
+def test_folded_head(cuda, B, T, H, V, cap):
+    g = torch.Generator().manual_seed(B + T + H + V)
+    hidden = torch.randn(B, T, H, generator=g).to(torch.bfloat16).to(cuda)
+    w = G.quantize_fp8((torch.randn(V, H, generator=g) * 3 / H ** 0.5).to(cuda), block=(128, 128))
+    ids = torch.randint(0, V, (B, T), generator=g, dtype=torch.int32).to(cuda)
+    edges = [0, V - 1] + [e for e in (127, 128, 255, 256, 511, 2047) if e < V]
+    ids.view(-1)[:min(len(edges), B * T)] = torch.tensor(edges[:B * T], dtype=torch.int32, device=cuda)
+    out = lm_head_forward(hidden, w, ids, cfg=G.LossConfig(softcap=cap))
+    torch.cuda.synchronize()
+    assert G.ops.check_device_status(out["problem"]) == 0
+    q = G.quantize_fp8(hidden.view(-1, H))
+    y, mag = R.product(q.values, q.scales, w.values, w.scales)
+    err = R.product_bound(y, mag, H)
+    if cap:
+        y = cap * torch.tanh(y / cap)
+        err = err + 2.6e-7 * cap
+    lse = torch.logsumexp(y, 1)
+    lp = y.gather(1, ids.view(-1).long()[:, None])[:, 0] - lse
+    p = torch.exp(y - lse[:, None])
+    ent = -(p * (y - lse[:, None])).sum(1)
+    worst = err.amax(1)
+    # a term of the sum: its exponent is rounded twice (2^-19 each while |y log2e| <= 64), ex2.approx 2^-22, and at
+    # most V / 64 + 600 additions in f32; the logarithm, the merged maximum and the result are f32 numbers below 64
+    e_sum = 3 * 2.0 ** -20 + 2.0 ** -22 + (min(V, 16384) / 64 + 600) * 2.0 ** -24 + 4 * 2.0 ** -19
+    R.assert_within(out["lse"].view(-1), lse, worst + e_sum, "lse")
+    R.assert_within(out["per_token_logps"].view(-1), lp, 2 * worst + e_sum, "log-probs")
+    # entropy = lse - U / S: U has the terms' relative error times |y|
+    R.assert_within(out["token_entropy"].view(-1), ent, 2 * worst * (1 + y.abs().amax(1)) + e_sum * (2 + (p * y.abs()).sum(1)), "entropy")
+
+
+def test_folded_head_feeds_the_loss_and_shards(cuda):
+    """The whole forward of the token loss on an 8-bit head equals the loss on its dequantised logits; two vocabulary
+    shards merged by hand give the unsharded log-probs."""
+    B, T, H, V = 2, 40, 256, 1536
+    g = torch.Generator().manual_seed(5)
+    hidden = torch.randn(B, T, H, generator=g).to(torch.bfloat16).to(cuda)
+    wt = (torch.randn(V, H, generator=g) * 0.2).to(cuda)
+    w = G.quantize_fp8(wt, block=(128, 128))
+    ids = torch.randint(0, V, (B, T), generator=g, dtype=torch.int32).to(cuda)
+    mask = (torch.rand(B, T, generator=g) < 0.7).float().to(cuda)
+    adv = torch.randn(B, generator=g).to(cuda)
+    old = lm_head_forward(hidden, w, ids)["per_token_logps"] + 0.1
+    out = lm_head_forward(hidden, w, ids, mask, adv, mask.sum(), old)
+    q = G.quantize_fp8(hidden.view(-1, H))
+    y = R.product(q.values, q.scales, w.values, w.scales)[0].view(B, T, V)
+    lp = torch.log_softmax(y, -1).gather(-1, ids.long()[..., None])[..., 0]
+    ratio = torch.exp(lp - old.double())
+    a = adv.double()[:, None]
+    loss = -(torch.minimum(ratio * a, ratio.clamp(0.8, 1.3) * a) * mask).sum() / mask.sum()
+    assert abs(float(out["loss"]) - float(loss)) <= 1e-4 * abs(float(loss)) + 1e-6
+    from mllm_jax_b200 import _lib
+    from mllm_jax_b200.fp8 import _bind
+    lib = _lib.load()
+    parts = []
+    for a0, b0 in ((0, 640), (640, V)):
+        shard = G.quantize_fp8(wt[a0:b0], block=(128, 128))
+        args = _bind(q, shard)
+        buf = torch.empty(lib.mllm_lm_head_fp8_partials_bytes(B * T, b0 - a0), dtype=torch.uint8, device=cuda)
+        args.vocab_start, args.vocab_total = a0, V
+        args.chosen_ids, args.partials = ids.data_ptr(), buf.data_ptr()
+        _lib.call("mllm_lm_head_fp8_partials", args, torch.cuda.current_stream().cuda_stream)
+        parts.append(buf[:16 * B * T].view(torch.float32).view(B * T, 4).double())
+    top = torch.maximum(parts[0][:, 0], parts[1][:, 0])
+    total = sum(p[:, 1] * torch.exp(p[:, 0] - top) for p in parts)
+    merged = sum(p[:, 3] for p in parts) - top - total.log()
+    assert (merged - lp.view(-1)).abs().max() <= 1e-4
+
+
+def test_streams_and_graph_replay(cuda):
+    for M in (4, 200):
+        x, w = _operands(M, 3000, 512, 90, cuda)
+        x2 = G.quantize_fp8(_x(M, 512, torch.bfloat16, 91, cuda))
+        want = [G.fp8_matmul(t, w) for t in (x, x2)]
+        torch.cuda.synchronize()
+        streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+        for _ in range(3):
+            for k, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[k] = G.fp8_matmul((x, x2)[k], w)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        raw = _x(M, 512, torch.bfloat16, 90, cuda, 0.5)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = G.fp8_matmul(raw, w)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0])
+        raw.copy_(_x(M, 512, torch.bfloat16, 91, cuda))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[1])
