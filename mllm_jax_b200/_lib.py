@@ -215,6 +215,23 @@ def call(name: str, args, stream: int) -> None:
                         lib.mllm_grpo_last_cuda_error().decode())
 
 
+def launch(name: str, args, device) -> None:
+    """`call` on the current stream of `device` (a CUDA torch.device with an index), whichever device is current.
+
+    A call of a few microseconds on the GPU is bound by the host: switching to a device that is already current and
+    wrapping its stream in an object cost 8 us of the 25 us that a small lookup took."""
+    from torch._C import _cuda_getCurrentRawStream, _cuda_getDevice
+
+    index = device.index
+    if _cuda_getDevice() == index:
+        call(name, args, _cuda_getCurrentRawStream(index))
+    else:
+        import torch
+
+        with torch.cuda.device(index):
+            call(name, args, _cuda_getCurrentRawStream(index))
+
+
 def launch_count() -> int:
     return int(load().mllm_grpo_launch_count())
 

@@ -11,10 +11,10 @@
 // bits first, which restores the middles and crosses none.  (For f32 inputs a quotient within 2^-19 of a middle
 // counts as the middle.)  A division per element would cost more than the memory traffic allows.
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include "grpo_common.cuh"
 #include "grpo_launch.h"
+#include "grpo_rowpass.cuh"
 
 namespace grpo {
 namespace fp8q {
@@ -23,6 +23,15 @@ constexpr int kThreads = 256;
 constexpr float kMost = 448.0f;
 constexpr float kLeast = 448.0f * 1.17549435e-38f;
 
+template <typename T>
+struct IsBf16 {
+  static constexpr bool value = false;
+};
+template <>
+struct IsBf16<__nv_bfloat16> {
+  static constexpr bool value = true;
+};
+
 struct Params {
   int64_t rows, cols, x_stride, q_stride, blocks;  // blocks along a row
   const void* x;
@@ -30,17 +39,93 @@ struct Params {
   float* scales;
 };
 
-__device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float up(__half v) { return __half2float(v); }
-__device__ __forceinline__ float up(float v) { return v; }
-
+// EV elements of x as raw 32-bit words: kept as they were read (two to a word for the 16-bit types) between the
+// maximum and the conversion, and the maximum is taken on pairs.  (Holding f32 values instead took 224 registers in
+// the 128 x 128 kernel, one CTA per SM: 815 us for a 151936 x 3584 weight.)
 template <typename T, int EV>
-struct alignas(sizeof(T) * EV) Vec {
-  T v[EV];
+struct Raw {
+  static constexpr int kBytes = int(sizeof(T)) * EV;
+  static constexpr int kWords = kBytes < 4 ? 1 : kBytes / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void load(const T* at) {
+    if constexpr (kBytes == 16) {
+      const uint4 v = ldg_stream(reinterpret_cast<const uint4*>(at));
+      w[0] = v.x;
+      w[1] = v.y;
+      w[2] = v.z;
+      w[3] = v.w;
+    } else if constexpr (kBytes == 8) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+      w[0] = v.x;
+      w[1] = v.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = __ldg(reinterpret_cast<const unsigned int*>(at));
+    } else {
+      w[0] = __ldg(reinterpret_cast<const unsigned short*>(at));
+    }
+  }
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[j]);
+    } else {
+      const uint16_t h = uint16_t(w[j / 2] >> (16 * (j & 1)));
+      if constexpr (IsBf16<T>::value)
+        return __uint_as_float(uint32_t(h) << 16);
+      else
+        return __half2float(__ushort_as_half(h));
+    }
+  }
 };
+
+// Running maximum of magnitudes that leaves NaNs out.
+template <typename T>
+struct AbsMax {
+  uint32_t m = 0u;  // f32 bits, or two 16-bit maxima
+  template <int EV>
+  __device__ __forceinline__ void add(const Raw<T, EV>& x) {
+#pragma unroll
+    for (int i = 0; i < Raw<T, EV>::kWords; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        m = __float_as_uint(fmaxf(__uint_as_float(m), fabsf(__uint_as_float(x.w[i]))));
+      } else if constexpr (IsBf16<T>::value) {
+        m = bf16x2_max(m, x.w[i] & 0x7fff7fffu);
+      } else {
+        asm("max.f16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(x.w[i] & 0x7fff7fffu));
+      }
+    }
+  }
+  __device__ __forceinline__ float value() const {
+    Raw<T, sizeof(T) == 4 ? 1 : 2> r;
+    r.w[0] = m;
+    if constexpr (sizeof(T) == 4)
+      return r.get(0);
+    else
+      return fmaxf(r.get(0), r.get(1));
+  }
+};
+
+// EV e4m3 bytes as one word.
 template <int EV>
-struct alignas(EV) Bytes {
-  uint8_t v[EV];
+struct Word;
+template <>
+struct Word<8> {
+  using type = uint2;
+};
+template <>
+struct Word<4> {
+  using type = uint32_t;
+};
+template <>
+struct Word<2> {
+  using type = uint16_t;
+};
+template <>
+struct Word<1> {
+  using type = uint8_t;
 };
 
 // y rounded to 19 bits: (33 y) - (33 y - y) keeps the upper part.
@@ -63,45 +148,48 @@ __device__ __forceinline__ float factor(float amax, float* scale) {
   return __fdiv_rn(kMost, top);
 }
 
-template <int EV, typename F>
-__device__ __forceinline__ Bytes<EV> convert(const F& value, float r) {
-  Bytes<EV> b;
-  if (EV == 1) {
-    b.v[0] = uint8_t(to_e4m3x2(snap(value(0) * r), 0.f));
+__device__ __forceinline__ uint32_t pair(float a, float b, float r) { return to_e4m3x2(snap(a * r), snap(b * r)); }
+template <typename T, int EV>
+__device__ __forceinline__ typename Word<EV>::type convert(const Raw<T, EV>& x, float r) {
+  if constexpr (EV == 8) {
+    return make_uint2(pair(x.get(0), x.get(1), r) | (pair(x.get(2), x.get(3), r) << 16),
+                      pair(x.get(4), x.get(5), r) | (pair(x.get(6), x.get(7), r) << 16));
+  } else if constexpr (EV == 4) {
+    return pair(x.get(0), x.get(1), r) | (pair(x.get(2), x.get(3), r) << 16);
+  } else if constexpr (EV == 2) {
+    return uint16_t(pair(x.get(0), x.get(1), r));
   } else {
-#pragma unroll
-    for (int j = 0; j < EV; j += 2) {
-      const uint16_t w = to_e4m3x2(snap(value(j) * r), snap(value(j + 1) * r));
-      b.v[j] = uint8_t(w);
-      b.v[j + 1] = uint8_t(w >> 8);
-    }
+    return uint8_t(pair(x.get(0), 0.f, r));
   }
-  return b;
 }
 
-// 1 x 128: 128 / EV consecutive threads hold a block (EV elements each; with one element a thread, 32 threads hold
-// four each, 32 apart).
+// 1 x 128: 128 / EV consecutive threads hold a block (EV elements each; with fewer elements a thread, 32 threads hold
+// several vectors each).
+template <typename T, int EV>
+struct RowGroup {
+  static constexpr int kThreadsPerBlock = 128 / EV > 32 ? 32 : 128 / EV;
+  static constexpr int kVecs = 128 / (kThreadsPerBlock * EV);
+};
 template <typename T, int EV>
 __global__ void __launch_bounds__(kThreads) row_blocks_kernel(const Params p) {
-  constexpr int G = EV == 1 ? 32 : (128 / EV > 32 ? 32 : 128 / EV);  // threads per block
-  constexpr int U = 128 / (G * EV);                                   // vectors per thread
+  constexpr int G = RowGroup<T, EV>::kThreadsPerBlock;
+  constexpr int U = RowGroup<T, EV>::kVecs;
   const int64_t g = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / G;  // block of the whole matrix
   const int l = threadIdx.x % G;
   const int64_t row = g / p.blocks, b = g - row * p.blocks;
   const bool in = row < p.rows;
   const int64_t c0 = b * 128;
   const T* x = static_cast<const T*>(p.x) + row * p.x_stride + c0;
-  Vec<T, EV> v[U];
-  float amax = 0.f;
+  Raw<T, EV> v[U];
+  AbsMax<T> top;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int c = (u * G + l) * EV;
-#pragma unroll
-    for (int j = 0; j < EV; ++j) v[u].v[j] = T(0.f);
-    if (in && c0 + c < p.cols) v[u] = *reinterpret_cast<const Vec<T, EV>*>(x + c);
-#pragma unroll
-    for (int j = 0; j < EV; ++j) amax = fmaxf(amax, fabsf(up(v[u].v[j])));
+    v[u].zero();
+    if (in && c0 + c < p.cols) v[u].load(x + c);
+    top.add(v[u]);
   }
+  float amax = top.value();
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   float scale;
@@ -112,34 +200,34 @@ __global__ void __launch_bounds__(kThreads) row_blocks_kernel(const Params p) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int c = (u * G + l) * EV;
-    if (c0 + c < p.cols)
-      *reinterpret_cast<Bytes<EV>*>(q + c) = convert<EV>([&](int j) { return up(v[u].v[j]); }, r);
+    if (c0 + c < p.cols) *reinterpret_cast<typename Word<EV>::type*>(q + c) = convert<T, EV>(v[u], r);
   }
 }
 
 // 128 x 128: one CTA per tile, the tile in registers.
 template <typename T, int EV>
-__global__ void __launch_bounds__(kThreads) tile_blocks_kernel(const Params p) {
-  constexpr int PER_ROW = 128 / EV;                    // vectors of a tile row
-  constexpr int U = 128 * PER_ROW / kThreads;          // vectors per thread
+__global__ void __launch_bounds__(kThreads, 16 * EV >= 64 && sizeof(T) == 2 ? 4 : 2) tile_blocks_kernel(const Params p) {
+  constexpr int PER_ROW = 128 / EV;            // vectors of a tile row
+  constexpr int U = 128 * PER_ROW / kThreads;  // vectors per thread
+  constexpr int STEP = kThreads / PER_ROW;     // rows between a thread's vectors
   __shared__ float red[kThreads / 32];
   const int64_t tr = blockIdx.x / p.blocks, tb = blockIdx.x - tr * p.blocks;
-  const int64_t r0 = tr * 128, c0 = tb * 128;
+  const int rr = threadIdx.x / PER_ROW, cc = (threadIdx.x % PER_ROW) * EV;
+  const int64_t r0 = tr * 128 + rr, c0 = tb * 128 + cc;
+  // vectors of this thread that are inside: its column is, and the first `mine` of its rows
+  const int64_t left = p.rows - r0;
+  const int mine = c0 < p.cols ? int(left <= 0 ? 0 : (left + STEP - 1) / STEP < U ? (left + STEP - 1) / STEP : U) : 0;
   const T* x = static_cast<const T*>(p.x) + r0 * p.x_stride + c0;
-  Vec<T, EV> v[U];
-  float amax = 0.f;
+  Raw<T, EV> v[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int i = u * kThreads + threadIdx.x, rr = i / PER_ROW, cc = (i % PER_ROW) * EV;
-#pragma unroll
-    for (int j = 0; j < EV; ++j) v[u].v[j] = T(0.f);
-    if (r0 + rr < p.rows && c0 + cc < p.cols) v[u] = *reinterpret_cast<const Vec<T, EV>*>(x + rr * p.x_stride + cc);
+    v[u].zero();
+    if (u < mine) v[u].load(x + u * (STEP * p.x_stride));
   }
+  AbsMax<T> top;
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int j = 0; j < EV; ++j) amax = fmaxf(amax, fabsf(up(v[u].v[j])));
-  amax = warp_max(amax);
+  for (int u = 0; u < U; ++u) top.add(v[u]);
+  float amax = warp_max(top.value());
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
   __syncthreads();
 #pragma unroll
@@ -149,17 +237,14 @@ __global__ void __launch_bounds__(kThreads) tile_blocks_kernel(const Params p) {
   if (threadIdx.x == 0) p.scales[blockIdx.x] = scale;
   uint8_t* q = p.q + r0 * p.q_stride + c0;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = u * kThreads + threadIdx.x, rr = i / PER_ROW, cc = (i % PER_ROW) * EV;
-    if (r0 + rr < p.rows && c0 + cc < p.cols)
-      *reinterpret_cast<Bytes<EV>*>(q + rr * p.q_stride + cc) = convert<EV>([&](int j) { return up(v[u].v[j]); }, r);
-  }
+  for (int u = 0; u < U; ++u)
+    if (u < mine) *reinterpret_cast<typename Word<EV>::type*>(q + u * (STEP * p.q_stride)) = convert<T, EV>(v[u], r);
 }
 
 template <typename T, int EV>
 static cudaError_t launch(const Params& p, int block_rows, cudaStream_t s) {
   if (block_rows == 1) {
-    constexpr int G = EV == 1 ? 32 : (128 / EV > 32 ? 32 : 128 / EV);
+    constexpr int G = RowGroup<T, EV>::kThreadsPerBlock;
     const int64_t groups = p.rows * p.blocks;
     row_blocks_kernel<T, EV><<<unsigned((groups + kThreads / G - 1) / (kThreads / G)), kThreads, 0, s>>>(p);
   } else {

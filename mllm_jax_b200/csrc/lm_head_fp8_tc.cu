@@ -8,10 +8,13 @@
 // One 128-byte row of the swizzled tiles holds exactly one block of 128 along K, so a pipeline stage is a block, and
 // its p_b (four tcgen05.mma of kind::f8f6f4, K = 32) is complete in tensor memory when the stage is read.  The scales
 // change from block to block and row to row, so the sum over blocks is formed in f32 registers: eight epilogue warps
-// fetch p_b with tcgen05.ld and add sx * sw * p_b, while the MMA warp fills the next accumulator.  320 threads:
-//   warp 0     TMA producer (x[128 x 128], w[BN x 128] per stage)
-//   warp 1     allocates tensor memory (512 columns = 512 / BN accumulators) and issues the MMAs from one thread
-//   warps 2-9  epilogue: warp -> (quarter of the 128 rows, half of the BN columns), thread = one row
+// fetch p_b with tcgen05.ld and add sx * sw * p_b, while the MMA warp fills the next accumulator.  384 threads:
+//   warp 0      TMA producer (x[128 x 128], w[BN x 128] per stage)
+//   warp 1      allocates tensor memory (512 columns = 512 / BN accumulators) and issues the MMAs from one thread
+//   warps 2, 3  idle (register budgets are set for whole warpgroups)
+//   warps 4-11  epilogue: warp -> (quarter of the 128 rows, half of the BN columns), thread = one row
+// An epilogue thread holds BN / 2 sums and 64 values on their way from tensor memory, more than the 168 registers that
+// 384 threads leave each: the first warpgroup gives registers up (setmaxnreg).
 #include "grpo_launch.h"
 #include "grpo_tc.cuh"
 #include "lm_head_fp8.h"
@@ -24,7 +27,10 @@ using namespace tc;
 constexpr int kBM = 128;
 constexpr int kBK = 128;
 constexpr int kStages = 4;
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
+// Registers per thread: at launch, then of the first warpgroup and of the two epilogue warpgroups.
+constexpr int kRegsLaunch = 168, kRegsFirst = 40, kRegsEpilogue = 224;
+static_assert(kRegsFirst * 128 + kRegsEpilogue * 256 <= kRegsLaunch * kThreads, "setmaxnreg.inc would wait forever");
 constexpr int kTmemCols = 512;
 constexpr int kABytes = kBM * kBK;
 
@@ -45,14 +51,13 @@ __device__ __forceinline__ void mma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t
 __host__ __device__ constexpr uint32_t instr_desc(int M, int N) {
   return (1u << 4) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr)
-      : "memory");
+template <int REGS>
+__device__ __forceinline__ void regs_give() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void regs_take() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
 // Store 8 f32 as consecutive elements of the output type.
@@ -159,9 +164,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_slot;
 
-  if (warp == 0) {
-    // ---------------- TMA producer ----------------
-    if (lane == 0) {
+  if (warp < 4) {
+    regs_give<kRegsFirst>();
+    if (warp == 0 && lane == 0) {
+      // ---------------- TMA producer ----------------
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -181,11 +187,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           }
         }
       }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
+    } else if (warp == 1 && lane == 0) {
+      // ---------------- MMA issuer ----------------
       constexpr uint32_t idesc = instr_desc(kBM, BN);
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
@@ -218,8 +221,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     __syncwarp();
   } else {
     // ---------------- epilogue ----------------
+    regs_take<kRegsEpilogue>();
     const int quarter = warp & 3;  // the TMEM lanes a warp may read: 32*(warp id mod 4) ...
-    const int half = (warp - 2) >> 2;
+    const int half = (warp - 4) >> 2;
     int buf = 0;
     uint32_t buf_phase = 0;
     bool ok = true;
@@ -257,16 +261,16 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         if (!ok) break;
         tc_fence_after();
         const uint32_t t_addr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(buf * BN + half * CW);
-        uint32_t v[2][16];
-        tmem_ld16(t_addr, v[0]);
+        uint32_t v[2][32];
+        tmem_ld32(t_addr, v[0]);
 #pragma unroll
-        for (int ch = 0; ch < CW / 16; ++ch) {
+        for (int ch = 0; ch < CW / 32; ++ch) {
           tmem_ld_wait();
-          if (ch + 1 < CW / 16) tmem_ld16(t_addr + uint32_t((ch + 1) * 16), v[(ch + 1) & 1]);
+          if (ch + 1 < CW / 32) tmem_ld32(t_addr + uint32_t((ch + 1) * 32), v[(ch + 1) & 1]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            acc[ch * 8 + j] = fma2(pack2(__uint_as_float(v[ch & 1][2 * j]), __uint_as_float(v[ch & 1][2 * j + 1])), f,
-                                   acc[ch * 8 + j]);
+          for (int j = 0; j < 16; ++j)
+            acc[ch * 16 + j] = fma2(pack2(__uint_as_float(v[ch & 1][2 * j]), __uint_as_float(v[ch & 1][2 * j + 1])), f,
+                                    acc[ch * 16 + j]);
         }
         tc_fence_before();
         __syncwarp();
@@ -427,6 +431,10 @@ static int launch_t(const Params& p, unsigned grid, const CUtensorMap& mx, const
   std::call_once(attr_once[dev], [&] {
     attr_err[dev] = cudaFuncSetAttribute(product_kernel<BN, STATS, O>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          int(Tile<BN>::kSmemBytes));
+    cudaFuncAttributes fa;
+    if (attr_err[dev] == cudaSuccess) attr_err[dev] = cudaFuncGetAttributes(&fa, product_kernel<BN, STATS, O>);
+    // the epilogue takes registers that the launch must have brought along
+    if (attr_err[dev] == cudaSuccess && fa.numRegs < kRegsLaunch) attr_err[dev] = cudaErrorInvalidConfiguration;
   });
   if (attr_err[dev] != cudaSuccess) return record_cuda_error(attr_err[dev]);
   product_kernel<BN, STATS, O><<<grid, kThreads, Tile<BN>::kSmemBytes, s>>>(mx, mw, p);

@@ -62,8 +62,7 @@ def _lookup(ids, weight, scale, vocab_start, vocab_total, device_status) -> torc
     a.weight_stride, a.token_stride = max(weight.stride(0), H), H
     a.dtype = _dtype(weight, "weight")
     a.ids, a.weight, a.out = ids32.data_ptr(), weight.data_ptr(), out.data_ptr()
-    with torch.cuda.device(dev):
-        _lib.call("mllm_grpo_embedding_lookup", a, torch.cuda.current_stream().cuda_stream)
+    _lib.launch("mllm_grpo_embedding_lookup", a, dev)
     return out
 
 
@@ -138,6 +137,5 @@ def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
         raise ValueError(f"{a.n_tokens} tokens of {H} are too many for one call")
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     a.ids, a.grad_out, a.dweight, a.workspace = ids32.data_ptr(), g.data_ptr(), res.data_ptr(), workspace.data_ptr()
-    with torch.cuda.device(dev):
-        _lib.call("mllm_grpo_embedding_grad", a, torch.cuda.current_stream().cuda_stream)
+    _lib.launch("mllm_grpo_embedding_grad", a, dev)
     return res

@@ -75,8 +75,7 @@ def quantize_fp8(x: torch.Tensor, *, block: Tuple[int, int] = (1, BLOCK)) -> Fp8
     a.rows, a.cols, a.x_stride, a.q_stride = R, C, max(x.stride(0), C), C
     a.block_rows, a.dtype = block[0], _DTYPES[x.dtype]
     a.x, a.q, a.scales = x.data_ptr(), values.data_ptr(), scales.data_ptr()
-    with torch.cuda.device(dev):
-        _lib.call("mllm_lm_head_fp8_quantize", a, torch.cuda.current_stream().cuda_stream)
+    _lib.launch("mllm_lm_head_fp8_quantize", a, dev)
     return Fp8Blocks(values, scales, block)
 
 
@@ -126,6 +125,5 @@ def fp8_matmul(x: Union[Fp8Blocks, torch.Tensor], w: Fp8Blocks, *, out_dtype: to
             (out.stride(1) != 1 and N > 1) or (M > 1 and out.stride(0) < N):
         raise ValueError(f"out must be [{M}, {N}] of bfloat16, float16 or float32 on {x.device} with contiguous rows")
     a.out_stride, a.out_dtype, a.out = max(out.stride(0), N) if M > 1 else N, _DTYPES[out.dtype], out.data_ptr()
-    with torch.cuda.device(x.device):
-        _lib.call("mllm_lm_head_fp8_matmul", a, torch.cuda.current_stream().cuda_stream)
+    _lib.launch("mllm_lm_head_fp8_matmul", a, x.device)
     return out

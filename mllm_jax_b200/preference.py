@@ -115,8 +115,7 @@ class PreferenceProblem:
         return dlogits
 
     def run(self, entry: str) -> None:
-        with torch.cuda.device(self.dev):
-            _lib.call(entry, self.a, torch.cuda.current_stream().cuda_stream)
+        _lib.launch(entry, self.a, self.dev)
 
     def outputs(self) -> dict:
         P = self.P
