@@ -55,14 +55,29 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// Bounded mbarrier wait shared by the three roles: false once any wait of the CTA has run out.
+// One try.  What these barriers order are asynchronous copies and tensor-memory accesses (with the tcgen05 fences), for
+// which the CTA's scope does; an acquire at cluster scope made every wait of a pipeline 3 % slower.
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// Bounded mbarrier wait shared by the three roles: false once any wait of the CTA has run out.  The clock is looked at
+// only after 64 tries (reading it takes longer than a barrier of a running pipeline stays closed).
 __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
-  if (cl::mbar_try(bar, parity)) return true;
+  if (try_wait(bar, parity)) return true;
   unsigned long long t0 = 0;
-  for (uint32_t spin = 0;; ++spin) {
-    if (cl::mbar_try(bar, parity)) return true;
-    if (*abort_flag) return false;
-    if ((spin & 255u) == 0) {
+  for (uint32_t spin = 1;; ++spin) {
+    if (try_wait(bar, parity)) return true;
+    if ((spin & 7u) == 0 && *abort_flag) return false;
+    if ((spin & 63u) == 0) {
       const unsigned long long now = cl::globaltimer();
       if (t0 == 0) t0 = now;
       if (now - t0 > kWaitNs) {

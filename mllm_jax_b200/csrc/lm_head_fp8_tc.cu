@@ -11,10 +11,24 @@
 // fetch p_b with tcgen05.ld and add sx * sw * p_b, while the MMA warp fills the next accumulator.  384 threads:
 //   warp 0      TMA producer (x[128 x 128], w[BN x 128] per stage)
 //   warp 1      allocates tensor memory (512 columns = 512 / BN accumulators) and issues the MMAs from one thread
-//   warps 2, 3  idle (register budgets are set for whole warpgroups)
-//   warps 4-11  epilogue: warp -> (quarter of the 128 rows, half of the BN columns), thread = one row
-// An epilogue thread holds BN / 2 sums and 64 values on their way from tensor memory, more than the 168 registers that
-// 384 threads leave each: the first warpgroup gives registers up (setmaxnreg).
+//   warps 2, 3  scales: sx * sw of the coming block for every row, through shared memory (a row's scales are contiguous
+//               along K: reading them in the epilogue touched 32 lines a load)
+//   warps 4-11  two epilogue warpgroups: warp -> a quarter of the 128 rows, thread = one row
+// An epilogue thread holds up to 128 sums and 64 values on their way from tensor memory, more than the 168 registers
+// that 384 threads leave each: the first warpgroup gives registers up (setmaxnreg).
+//
+// With BN = 256 there are two accumulators, and what bounds the kernel is the way from a commit through the epilogue
+// back to the MMA warp: the epilogue releases an accumulator as soon as its last values are in registers, before it
+// adds them.  (Four accumulators of 128 columns, multiplied separately, would leave more time, but a pair's MMA of 128
+// columns takes as long as one of 256.)  BN = 128 serves problems with fewer tiles than SMs.
+//
+// CTAS = 1: a CTA computes its tile by itself.  CTAS = 2: two CTAs of a cluster on neighbouring SMs compute 256 x 256
+// together (tcgen05 cta_group::2): each loads its own 128 rows of x and HALF of the weight tile, the tensor cores read
+// both halves.  With one CTA per 128 x 256 tile an SM asks L2 for 48 KB per block of 512 MMA cycles, more than L2
+// delivers (measured without any epilogue work: 914 cycles per block); the pair asks for 32 KB each.
+//
+// The finished tile goes through shared memory and leaves by TMA while the next one is accumulated (threads writing
+// their own rows: 4096 cycles per tile; coalesced stores from shared memory: 3300).
 #include "grpo_launch.h"
 #include "grpo_tc.cuh"
 #include "lm_head_fp8.h"
@@ -26,7 +40,6 @@ using namespace tc;
 
 constexpr int kBM = 128;
 constexpr int kBK = 128;
-constexpr int kStages = 4;
 constexpr int kThreads = 384;
 // Registers per thread: at launch, then of the first warpgroup and of the two epilogue warpgroups.
 constexpr int kRegsLaunch = 168, kRegsFirst = 40, kRegsEpilogue = 224;
@@ -34,18 +47,86 @@ static_assert(kRegsFirst * 128 + kRegsEpilogue * 256 <= kRegsLaunch * kThreads, 
 constexpr int kTmemCols = 512;
 constexpr int kABytes = kBM * kBK;
 
-template <int BN>
+constexpr int kBarBytes = 256;
+
+template <int BN, int CTAS>
 struct Tile {
-  static constexpr int kStageBytes = kABytes + BN * kBK;
-  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + 1024 /* alignment slack */ + 256 /* barriers */;
+  static constexpr int kBufs = kTmemCols / BN;  // accumulators
+  static constexpr int kBRows = BN / CTAS;      // weight rows that one CTA loads
+  static constexpr int kStageBytes = kABytes + kBRows * kBK;
+  static constexpr int kStages = kStageBytes > 32768 ? 3 : 4;
+  static constexpr int CW = BN / 2;             // columns of an epilogue warp
+  static constexpr int kHalves = BN / 128;      // blocks of weight rows in a tile
+  static constexpr int kScaleBytes = kBufs * kHalves * kBM * 4;
+  static constexpr int kStoreBytes = 32 * CW * 2;  // per epilogue warp: 32 rows of bf16 on their way out
+  static constexpr size_t kSmemBytes = 1024 /* alignment slack */ + size_t(kStages) * kStageBytes + 8 * kStoreBytes + kBarBytes +
+                                       kScaleBytes;
+  static_assert(kSmemBytes <= 227 * 1024, "");
+  // barriers: full[kStages], empty[kStages], then per accumulator: full, empty (the MMA warp's), slot_empty (the scale
+  // warps')
+  static_assert((2 * kStages + 3 * kBufs) * 8 <= kBarBytes, "");
 };
 
+template <int CTAS>
 __device__ __forceinline__ void mma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
+  if constexpr (CTAS == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrives at the barrier (of both CTAs of a pair) when the MMAs issued so far are done.
+template <int CTAS>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CTAS == 1)
+    mma_commit(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(uint16_t(3))
+        : "memory");
+}
+// Tile load into this CTA's shared memory; for a pair the barrier is the leader's.
+template <int CTAS>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  if constexpr (CTAS == 1)
+    tma_load_2d(dst, map, c0, c1, bar);
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+        "[%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+// Arrival at a barrier of the pair's leader.  What it releases are tensor-memory reads, which tcgen05.wait and the
+// fence before it have ordered: the default scope (the CTA) does.  A release at cluster scope waits for every store
+// of the thread as well and doubled the kernel's time.
+__device__ __forceinline__ void arrive_leader(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cl::map_to_cta(bar, 0)) : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot) {
+  if constexpr (CTAS == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(uint32_t(kTmemCols)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(uint32_t(kTmemCols)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_free(uint32_t base) {
+  if constexpr (CTAS == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(uint32_t(kTmemCols)) : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(uint32_t(kTmemCols)) : "memory");
 }
 // Instruction descriptor: D f32 (bit 4), A and B e4m3 (0), both K-major, N/8 at bits 17-22, M/16 at bits 24-28.
 __host__ __device__ constexpr uint32_t instr_desc(int M, int N) {
@@ -60,82 +141,168 @@ __device__ __forceinline__ void regs_take() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
-// Store 8 f32 as consecutive elements of the output type.
+// 16 bytes of output from the f32 pairs that hold them.
 template <typename O>
-__device__ __forceinline__ void store8(O* to, const float (&v)[8]);
+struct Out;
 template <>
-__device__ __forceinline__ void store8<float>(float* to, const float (&v)[8]) {
-  *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+struct Out<float> {
+  static constexpr int kPerVec = 4;
+  static __device__ __forceinline__ uint4 pack(const f32x2* v) {
+    uint4 o;
+    float a, b;
+    unpack2(v[0], a, b);
+    o.x = __float_as_uint(a);
+    o.y = __float_as_uint(b);
+    unpack2(v[1], a, b);
+    o.z = __float_as_uint(a);
+    o.w = __float_as_uint(b);
+    return o;
+  }
+};
+template <>
+struct Out<__nv_bfloat16> {
+  static constexpr int kPerVec = 8;
+  static __device__ __forceinline__ uint32_t two(f32x2 v) {
+    float a, b;
+    unpack2(v, a, b);
+    return pack_bf16x2(a, b);
+  }
+  static __device__ __forceinline__ uint4 pack(const f32x2* v) { return make_uint4(two(v[0]), two(v[1]), two(v[2]), two(v[3])); }
+};
+template <>
+struct Out<__half> {
+  static constexpr int kPerVec = 8;
+  static __device__ __forceinline__ uint32_t two(f32x2 v) {
+    float a, b;
+    unpack2(v, a, b);
+    return cl::pack_f16x2(a, b);
+  }
+  static __device__ __forceinline__ uint4 pack(const f32x2* v) { return make_uint4(two(v[0]), two(v[1]), two(v[2]), two(v[3])); }
+};
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int c1, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-template <>
-__device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* to, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                                             pack_bf16x2(v[6], v[7]));
-}
-template <>
-__device__ __forceinline__ void store8<__half>(__half* to, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(to) = make_uint4(cl::pack_f16x2(v[0], v[1]), cl::pack_f16x2(v[2], v[3]),
-                                             cl::pack_f16x2(v[4], v[5]), cl::pack_f16x2(v[6], v[7]));
-}
-template <typename O>
-__device__ __forceinline__ O down(float v);
-template <>
-__device__ __forceinline__ float down<float>(float v) {
-  return v;
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 down<__nv_bfloat16>(float v) {
-  return __float2bfloat16_rn(v);
-}
-template <>
-__device__ __forceinline__ __half down<__half>(float v) {
-  return __float2half_rn(v);
+
+// Writes a warp's 32 rows x CW columns, each thread holding a row.  Boxes of 32 rows x 128 bytes in shared memory, laid
+// out as TMA's 128-byte swizzle has them (16-byte chunk c of row r at c ^ (r mod 8): no bank conflicts), go out
+// asynchronously; columns and rows past the output are cut off by the tensor map, columns in steps of 16 bytes.  Rows
+// that do not start on 16-byte boundaries, and a last tile that ends inside 16 bytes (the cut would write the rest of
+// them), are written from there by ordinary stores, consecutive lanes taking consecutive elements.
+template <typename O, int CW, int BYTES>
+__device__ __forceinline__ void store_rows(const Params& p, const CUtensorMap* map, const f32x2 (&acc)[CW / 2], int64_t row0,
+                                           int64_t n0, int valid, uint32_t buf, int lane) {
+  constexpr int PV = Out<O>::kPerVec;       // elements of a 16-byte chunk
+  constexpr int BOX = 8 * PV;               // columns of a box
+  constexpr int ROOM = BYTES / (32 * 128);  // boxes that fit the warp's buffer
+  if (valid <= 0 || row0 >= p.n_rows) return;
+#pragma unroll
+  for (int c0 = 0; c0 < CW; c0 += BOX) {
+    if (c0 >= valid) break;  // uniform over the warp
+    constexpr int LAST = CW / BOX - 1;
+    const int at = (c0 / BOX) % ROOM;
+    if (at == 0) {
+      // the stores that last used this buffer have been read
+      if (lane == 0) cl::bulk_wait_read();
+      __syncwarp();
+    }
+    const uint32_t box = buf + uint32_t(at) * (32 * 128);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      cl::sts128(box + uint32_t(lane * 128 + ((k ^ (lane & 7)) << 4)), Out<O>::pack(&acc[(c0 + k * PV) / 2]));
+    if (p.out_aligned && (valid == CW || valid % PV == 0)) {
+      // one fence for the boxes that fit the buffer
+      if (at != ROOM - 1 && c0 / BOX != LAST && c0 + BOX < valid) continue;
+      cl::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < ROOM; ++i)
+          if (i <= at) tma_store_2d(map, int(n0) + c0 - (at - i) * BOX, int(row0), buf + uint32_t(i) * (32 * 128));
+      }
+    } else {
+      __syncwarp();
+      constexpr int RPI = BOX >= 32 ? 1 : 32 / BOX;  // rows per iteration
+      O* const out = static_cast<O*>(p.out) + n0 + c0;
+#pragma unroll
+      for (int e0 = 0; e0 < BOX; e0 += 32) {
+        const int e = e0 + lane % (BOX < 32 ? BOX : 32), k = e / PV;
+#pragma unroll 4
+        for (int r = BOX < 32 ? lane / BOX : 0; r < 32; r += RPI) {
+          const uint32_t at = box + uint32_t(r * 128 + ((k ^ (r & 7)) << 4) + (e % PV) * int(sizeof(O)));
+          if (row0 + r < p.n_rows && c0 + e < valid) {
+            O* to = out + (row0 + r) * p.out_stride + e;
+            if constexpr (sizeof(O) == 4) {
+              uint32_t v;
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+              *reinterpret_cast<uint32_t*>(to) = v;
+            } else {
+              uint16_t v;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+              *reinterpret_cast<uint16_t*>(to) = v;
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
 }
 
 // STATS: fold the tiles into (max, sumexp, sum e*y, chosen) instead of writing them as O.
-template <int BN, bool STATS, typename O>
+template <int BN, int CTAS, bool STATS, typename O>
 __global__ void __launch_bounds__(kThreads, 1)
-product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Params p) {
-  constexpr int kBufs = kTmemCols / BN;
-  constexpr int CW = BN / 2;  // columns of an epilogue warp
-  constexpr int kStageBytes = Tile<BN>::kStageBytes;
+product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+               const __grid_constant__ CUtensorMap map_out, const Params p) {
+  using T = Tile<BN, CTAS>;
+  constexpr int kHalves = T::kHalves, kBufs = T::kBufs, kStages = T::kStages, kStageBytes = T::kStageBytes;
+  constexpr int CW = T::CW;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = cl::smem_u32(smem_raw);
   const uint32_t tiles = (raw + 1023u) & ~1023u;
-  const uint32_t bars = tiles + uint32_t(kStages) * kStageBytes;
+  const uint32_t store_buf = tiles + uint32_t(kStages) * kStageBytes;
+  const uint32_t bars = store_buf + 8u * T::kStoreBytes;
   auto full_bar = [&](int s) { return bars + 8u * uint32_t(s); };
   auto empty_bar = [&](int s) { return bars + 8u * uint32_t(kStages + s); };
   auto acc_full = [&](int a) { return bars + 8u * uint32_t(2 * kStages + a); };
   auto acc_empty = [&](int a) { return bars + 8u * uint32_t(2 * kStages + kBufs + a); };
+  auto slot_empty = [&](int a) { return bars + 8u * uint32_t(2 * kStages + 2 * kBufs + a); };
+  float* const scales = reinterpret_cast<float*>(smem_raw + (bars - raw) + kBarBytes);  // [accumulator][half][row]
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = CTAS == 1 ? 0 : int(cl::cluster_rank());
+  const int team = int(blockIdx.x) / CTAS, teams = int(gridDim.x) / CTAS;
 
-  // Work of this CTA: `n_mine` tiles.  Tiles (or, folded, runs of tiles of one row tile) are numbered so that the
-  // CTAs that run together take up to 16 row tiles of the same weight tile, which L2 then serves to all of them.
+  // Work of this CTA (pair): `n_mine` tiles.  Tiles (or, folded, runs of tiles of the same rows) are numbered so that
+  // the CTAs that run together take up to 2048 rows of the same weight tile, which L2 then serves to all of them.
+  constexpr int kGroup = 16 / CTAS;
   const int units = STATS ? p.splits : p.n_tiles;
+  const int m_teams = (p.m_tiles + CTAS - 1) / CTAS;
   auto place = [&](int unit_id, int* m_tile, int* unit) {
-    const int per_group = 16 * units;
+    const int per_group = kGroup * units;
     const int group = unit_id / per_group, within = unit_id - group * per_group;
-    const int rows_in_group = min(16, p.m_tiles - group * 16);
-    *m_tile = group * 16 + within % rows_in_group;
+    const int rows_in_group = min(kGroup, m_teams - group * kGroup);
+    *m_tile = (group * kGroup + within % rows_in_group) * CTAS + rank;
     *unit = within / rows_in_group;
   };
   int m_fixed = 0, split = 0, n_mine;
   if (STATS) {
-    place(blockIdx.x, &m_fixed, &split);
+    place(team, &m_fixed, &split);
     n_mine = max(0, min(p.tiles_per_split, p.n_tiles - split * p.tiles_per_split));
   } else {
-    n_mine = (p.m_tiles * p.n_tiles - int(blockIdx.x) + int(gridDim.x) - 1) / int(gridDim.x);
+    n_mine = (m_teams * p.n_tiles - team + teams - 1) / teams;
   }
   auto tile_at = [&](int i, int* m_tile, int* n_tile) {
     if (STATS) {
       *m_tile = m_fixed;
       *n_tile = split * p.tiles_per_split + i;
     } else {
-      place(int(blockIdx.x) + i * int(gridDim.x), m_tile, n_tile);
+      place(team + i * teams, m_tile, n_tile);
     }
   };
 
@@ -146,21 +313,20 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       cl::mbar_init(empty_bar(s), 1);
     }
     for (int a = 0; a < kBufs; ++a) {
-      cl::mbar_init(acc_full(a), 1);
-      cl::mbar_init(acc_empty(a), 8);  // one arrival per epilogue warp
+      cl::mbar_init(acc_full(a), 3);          // the MMAs' commit and both scale warps
+      cl::mbar_init(acc_empty(a), 8 * CTAS);  // one arrival per epilogue warp (of both CTAs, in the leader)
+      cl::mbar_init(slot_empty(a), 8);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_tmap(&map_x);
     prefetch_tmap(&map_w);
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(cl::smem_u32(&tmem_base_slot)),
-                 "r"(uint32_t(kTmemCols))
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  if (warp == 1) tmem_alloc<CTAS>(cl::smem_u32(&tmem_base_slot));
   tc_fence_before();
-  __syncthreads();
+  if (CTAS == 1)
+    __syncthreads();
+  else
+    cl::cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_slot;
 
@@ -178,35 +344,47 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           ok = wait_or_abort(empty_bar(stage), phase ^ 1u, &abort_flag, p.device_status);
           if (!ok) break;
           const uint32_t a_dst = tiles + uint32_t(stage) * kStageBytes;
-          cl::mbar_expect_tx(full_bar(stage), uint32_t(kStageBytes));
-          tma_load_2d(a_dst, &map_x, kb * kBK, m_tile * kBM, full_bar(stage));
-          tma_load_2d(a_dst + kABytes, &map_w, kb * kBK, n_tile * BN, full_bar(stage));
+          // the bytes of both CTAs are counted at the leader's barrier
+          if (rank == 0) cl::mbar_expect_tx(full_bar(stage), uint32_t(CTAS * kStageBytes));
+          const uint32_t bar = CTAS == 1 ? full_bar(stage) : cl::map_to_cta(full_bar(stage), 0);
+          load_tile<CTAS>(a_dst, &map_x, kb * kBK, m_tile * kBM, bar);
+          load_tile<CTAS>(a_dst + kABytes, &map_w, kb * kBK, n_tile * BN + rank * T::kBRows, bar);
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-    } else if (warp == 1 && lane == 0) {
-      // ---------------- MMA issuer ----------------
-      constexpr uint32_t idesc = instr_desc(kBM, BN);
+      // the stages' last releases come from the leader's tensor core: none may be on its way when this CTA leaves
+      for (int i = 0; i < kStages && ok; ++i) {
+        ok = wait_or_abort(empty_bar(stage), phase ^ 1u, &abort_flag, p.device_status);
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      // ---------------- MMA issuer (the leader's) ----------------
+      constexpr uint32_t idesc = instr_desc(kBM * CTAS, BN);
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
       bool ok = true;
       for (int t = 0; t < n_mine && ok; ++t) {
         for (int kb = 0; kb < p.k_blocks; ++kb) {
-          ok = wait_or_abort(acc_empty(buf), buf_phase ^ 1u, &abort_flag, p.device_status) &&
-               wait_or_abort(full_bar(stage), phase, &abort_flag, p.device_status);
+          // the tiles are there long before the accumulator is free: that wait comes last, with everything prepared
+          ok = wait_or_abort(full_bar(stage), phase, &abort_flag, p.device_status);
           if (!ok) break;
-          tc_fence_after();
           const uint32_t a_src = tiles + uint32_t(stage) * kStageBytes;
           const uint64_t adesc = smem_desc(a_src), bdesc = smem_desc(a_src + kABytes);
           const uint32_t d_addr = tmem_base + uint32_t(buf * BN);
+          ok = wait_or_abort(acc_empty(buf), buf_phase ^ 1u, &abort_flag, p.device_status);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kBK / 32; ++k)  // 32 bytes further along K inside the swizzled row: +2 in the address field
-            mma_f8(d_addr, adesc + uint64_t(2 * k), bdesc + uint64_t(2 * k), idesc, k != 0 ? 1u : 0u);
-          mma_commit(empty_bar(stage));
-          mma_commit(acc_full(buf));
+            mma_f8<CTAS>(d_addr, adesc + uint64_t(2 * k), bdesc + uint64_t(2 * k), idesc, k != 0 ? 1u : 0u);
+          commit<CTAS>(acc_full(buf));
+          commit<CTAS>(empty_bar(stage));
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
@@ -217,13 +395,62 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           }
         }
       }
+    } else if (warp >= 2) {
+      // ---------------- scales ----------------
+      int buf = 0;
+      uint32_t buf_phase = 0;
+      bool ok = true;
+      for (int t = 0; t < n_mine && ok; ++t) {
+        int m_tile, n_tile;
+        tile_at(t, &m_tile, &n_tile);
+        const int r0 = (warp - 2) * 64 + lane;
+        const int64_t row = int64_t(m_tile) * kBM + r0, n0 = int64_t(n_tile) * BN;
+        const float* sx0 = p.x_scales + (row < p.n_rows ? row : p.n_rows - 1) * p.k_blocks;
+        const float* sx1 = p.x_scales + (row + 32 < p.n_rows ? row + 32 : p.n_rows - 1) * p.k_blocks;
+        const float* sw[kHalves];
+        float w[kHalves];
+#pragma unroll
+        for (int g = 0; g < kHalves; ++g) {
+          // columns past the vocabulary have no scales: whatever they get is cut off
+          sw[g] = p.w_scales + (n0 + g * 128 < p.vocab ? n0 + g * 128 : n0) / 128 * p.k_blocks;
+          w[g] = sw[g][0];
+        }
+        float x0 = sx0[0], x1 = sx1[0];
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          float a0[kHalves], a1[kHalves];
+#pragma unroll
+          for (int g = 0; g < kHalves; ++g) {
+            a0[g] = x0 * w[g];
+            a1[g] = x1 * w[g];
+          }
+          if (kb + 1 < p.k_blocks) {
+            x0 = sx0[kb + 1];
+            x1 = sx1[kb + 1];
+#pragma unroll
+            for (int g = 0; g < kHalves; ++g) w[g] = sw[g][kb + 1];
+          }
+          ok = wait_or_abort(slot_empty(buf), buf_phase ^ 1u, &abort_flag, p.device_status);
+          if (!ok) break;
+#pragma unroll
+          for (int g = 0; g < kHalves; ++g) {
+            scales[(buf * kHalves + g) * kBM + r0] = a0[g];
+            scales[(buf * kHalves + g) * kBM + r0 + 32] = a1[g];
+          }
+          __syncwarp();
+          if (lane == 0) cl::mbar_arrive(acc_full(buf));
+          if (++buf == kBufs) {
+            buf = 0;
+            buf_phase ^= 1u;
+          }
+        }
+      }
     }
-    __syncwarp();
   } else {
     // ---------------- epilogue ----------------
     regs_take<kRegsEpilogue>();
     const int quarter = warp & 3;  // the TMEM lanes a warp may read: 32*(warp id mod 4) ...
     const int half = (warp - 4) >> 2;
+    const uint32_t my_store = store_buf + uint32_t(warp - 4) * T::kStoreBytes;
     int buf = 0;
     uint32_t buf_phase = 0;
     bool ok = true;
@@ -245,36 +472,43 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     for (int t = 0; t < n_mine && ok; ++t) {
       int m_tile, n_tile;
       tile_at(t, &m_tile, &n_tile);
-      const int64_t row = int64_t(m_tile) * kBM + quarter * 32 + lane;
       const int64_t n0 = int64_t(n_tile) * BN + half * CW;
-      // scales of this thread's row and of this warp's columns (one block of 128 weight rows or part of it)
-      const float* sx = p.x_scales + (row < p.n_rows ? row : p.n_rows - 1) * p.k_blocks;
-      const float* sw = p.w_scales + (n0 < p.vocab ? n0 / 128 : 0) * p.k_blocks;
       f32x2 acc[CW / 2];
 #pragma unroll
       for (int j = 0; j < CW / 2; ++j) acc[j] = 0ull;
-      float f_next = sx[0] * sw[0];
       for (int kb = 0; kb < p.k_blocks; ++kb) {
-        const f32x2 f = pack2(f_next, f_next);
-        if (kb + 1 < p.k_blocks) f_next = sx[kb + 1] * sw[kb + 1];
         ok = wait_or_abort(acc_full(buf), buf_phase, &abort_flag, p.device_status);
         if (!ok) break;
         tc_fence_after();
         const uint32_t t_addr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(buf * BN + half * CW);
         uint32_t v[2][32];
         tmem_ld32(t_addr, v[0]);
+        tmem_ld32(t_addr + 32u, v[1]);
+        const float scale = scales[(buf * kHalves + half % kHalves) * kBM + quarter * 32 + lane];
+        const f32x2 f = pack2(scale, scale);
 #pragma unroll
         for (int ch = 0; ch < CW / 32; ++ch) {
-          tmem_ld_wait();
-          if (ch + 1 < CW / 32) tmem_ld32(t_addr + uint32_t((ch + 1) * 32), v[(ch + 1) & 1]);
+          if ((ch & 1) == 0) {
+            tmem_ld_wait();  // two chunks of 32 columns per wait
+            if (ch + 2 >= CW / 32) {
+              // everything of this accumulator is in registers: hand it back
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                if (CTAS == 1)
+                  cl::mbar_arrive(acc_empty(buf));
+                else
+                  arrive_leader(acc_empty(buf));
+                cl::mbar_arrive(slot_empty(buf));
+              }
+            }
+          }
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             acc[ch * 16 + j] = fma2(pack2(__uint_as_float(v[ch & 1][2 * j]), __uint_as_float(v[ch & 1][2 * j + 1])), f,
                                     acc[ch * 16 + j]);
+          if (ch + 2 < CW / 32) tmem_ld32(t_addr + uint32_t((ch + 2) * 32), v[ch & 1]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) cl::mbar_arrive(acc_empty(buf));
         if (++buf == kBufs) {
           buf = 0;
           buf_phase ^= 1u;
@@ -283,22 +517,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       if (!ok) break;
       const int valid = int(p.vocab - n0 < CW ? (p.vocab - n0 > 0 ? p.vocab - n0 : 0) : CW);
       if (!STATS) {
-        if (row < p.n_rows) {
-          O* out = static_cast<O*>(p.out) + row * p.out_stride + n0;
-#pragma unroll
-          for (int j = 0; j < CW / 8; ++j) {
-            float y[8];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) unpack2(acc[j * 4 + q], y[2 * q], y[2 * q + 1]);
-            if (p.out_aligned && j * 8 + 8 <= valid) {
-              store8<O>(out + j * 8, y);
-            } else {
-#pragma unroll
-              for (int q = 0; q < 8; ++q)
-                if (j * 8 + q < valid) out[j * 8 + q] = down<O>(y[q]);
-            }
-          }
-        }
+        store_rows<O, CW, T::kStoreBytes>(p, &map_out, acc, int64_t(m_tile) * kBM + quarter * 32, n0, valid, my_store, lane);
       } else if (valid > 0) {
         const int64_t c_local = c >= 0 ? c - n0 : -1;
         float y[CW];
@@ -339,18 +558,24 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       if (row < p.n_rows)
         p.partials[(int64_t(split) * 2 + half + 1) * p.n_rows + row] =
             ok ? make_float4(m, s, u, yc) : make_float4(kNegInit, 0.f, 0.f, 0.f);
+    } else if (lane == 0) {
+      cl::bulk_wait_all();  // the buffers are read and written out before this CTA's shared memory goes
     }
   }
 
   // ---------------- teardown: every role arrives here, also after an abort ----------------
+  __syncwarp();
+  if (abort_flag && warp == 1) {
+    for (int i = 0; i < 4; ++i) __nanosleep(500000);  // copies or MMAs may still be in flight: bounded time for them
+  }
   tc_fence_before();
-  __syncthreads();
+  if (CTAS == 1)
+    __syncthreads();
+  else
+    cl::cluster_sync_all();  // neither CTA leaves while the other may signal its barriers or read its tiles
   if (warp == 1) {
-    if (abort_flag) {
-      for (int i = 0; i < 4; ++i) __nanosleep(500000);  // copies or MMAs may still be in flight: bounded time for them
-    }
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(uint32_t(kTmemCols)) : "memory");
+    tmem_free<CTAS>(tmem_base);
   }
 }
 
@@ -383,92 +608,114 @@ __global__ void __launch_bounds__(256) merge_kernel(float4* partials, int64_t n_
   }
 }
 
-// e4m3 [rows, cols] with `ld` bytes between rows -> boxes of box_rows x 128 bytes, 128-byte swizzle, zeros outside.
-static bool make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+// [rows, cols] of `elem` bytes with `ld` bytes between rows -> boxes of box_rows x 128 bytes, 128-byte swizzle, zeros
+// outside.
+static bool make_map(CUtensorMap* map, CUtensorMapDataType type, int elem, const void* base, int64_t rows, int64_t cols,
+                     int64_t ld, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
   const cuuint64_t strides[1] = {cuuint64_t(ld)};
-  const cuuint32_t box[2] = {cuuint32_t(kBK), cuuint32_t(box_rows)};
+  const cuuint32_t box[2] = {cuuint32_t(128 / elem), cuuint32_t(box_rows)};
   const cuuint32_t estr[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+  return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 constexpr int kSms = 148;
+constexpr int kFoldBN = 256;
 
-// Column ranges of the folded form: as many whole tiles per CTA as balance the SMs best (each CTA costs about a
-// third of a tile to start and end).
-static int fold_tiles_per_split(int64_t m_tiles, int64_t n_tiles) {
+// Pairs of CTAs from two row tiles on: half of a pair would idle with one.
+static int ctas_for(int64_t m_tiles) { return m_tiles >= 2 ? 2 : 1; }
+
+// Column ranges of the folded form: as many whole tiles per CTA (pair) as balance the SMs best; each costs about a
+// third of a tile to start and end.
+static void fold_plan(int64_t n_rows, int64_t vocab, int* tiles_per_split, int* splits) {
+  const int64_t m_tiles = (n_rows + kBM - 1) / kBM, n_tiles = (vocab + kFoldBN - 1) / kFoldBN;
+  const int ctas = ctas_for(m_tiles);
+  const int64_t m_teams = (m_tiles + ctas - 1) / ctas, slots = kSms / ctas;
   double best = 1e300;
   int64_t pick = 1;
   for (int64_t per = 1; per <= n_tiles && per <= 64; ++per) {
-    const int64_t ctas = m_tiles * ((n_tiles + per - 1) / per);
-    const double cost = double((ctas + kSms - 1) / kSms) * (double(per) + 0.33);
+    const int64_t teams = m_teams * ((n_tiles + per - 1) / per);
+    const double cost = double((teams + slots - 1) / slots) * (double(per) + 0.33);
     if (cost < best * 0.999) {
       best = cost;
       pick = per;
     }
   }
-  return int(pick);
+  *tiles_per_split = int(pick);
+  *splits = int((n_tiles + pick - 1) / pick);
 }
 
-constexpr int kFoldBN = 256;
-
-static void fold_plan(int64_t n_rows, int64_t vocab, int* tiles_per_split, int* splits) {
-  const int64_t m_tiles = (n_rows + kBM - 1) / kBM, n_tiles = (vocab + kFoldBN - 1) / kFoldBN;
-  *tiles_per_split = fold_tiles_per_split(m_tiles, n_tiles);
-  *splits = int((n_tiles + *tiles_per_split - 1) / *tiles_per_split);
-}
-
-template <int BN, bool STATS, typename O>
-static int launch_t(const Params& p, unsigned grid, const CUtensorMap& mx, const CUtensorMap& mw, cudaStream_t s) {
+template <int BN, int CTAS, bool STATS, typename O>
+static int launch_t(const Params& p, unsigned grid, const CUtensorMap& mx, const CUtensorMap& mw,
+                    const CUtensorMap& mo, cudaStream_t s) {
+  using T = Tile<BN, CTAS>;
+  auto* kernel = product_kernel<BN, CTAS, STATS, O>;
   static std::once_flag attr_once[64];
   static cudaError_t attr_err[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MLLM_GRPO_ERR_NO_DEVICE;
   std::call_once(attr_once[dev], [&] {
-    attr_err[dev] = cudaFuncSetAttribute(product_kernel<BN, STATS, O>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         int(Tile<BN>::kSmemBytes));
+    attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(T::kSmemBytes));
     cudaFuncAttributes fa;
-    if (attr_err[dev] == cudaSuccess) attr_err[dev] = cudaFuncGetAttributes(&fa, product_kernel<BN, STATS, O>);
+    if (attr_err[dev] == cudaSuccess) attr_err[dev] = cudaFuncGetAttributes(&fa, kernel);
     // the epilogue takes registers that the launch must have brought along
     if (attr_err[dev] == cudaSuccess && fa.numRegs < kRegsLaunch) attr_err[dev] = cudaErrorInvalidConfiguration;
   });
   if (attr_err[dev] != cudaSuccess) return record_cuda_error(attr_err[dev]);
-  product_kernel<BN, STATS, O><<<grid, kThreads, Tile<BN>::kSmemBytes, s>>>(mx, mw, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = T::kSmemBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CTAS;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CTAS > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, mo, p);
   count_launch();
-  const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);
 }
 
-template <int BN, bool STATS, typename O>
+template <int BN, int CTAS, bool STATS, typename O>
 static int launch(Params p, const mllm_lm_head_fp8_args* a, cudaStream_t s) {
   p.m_tiles = int((p.n_rows + kBM - 1) / kBM);
   p.n_tiles = int((p.vocab + BN - 1) / BN);
-  CUtensorMap mx, mw;
-  if (!make_map(&mx, a->hidden, a->n_rows, a->hidden_dim, a->hidden_stride, kBM) ||
-      !make_map(&mw, a->weight, a->vocab, a->hidden_dim, a->weight_stride, BN))
+  CUtensorMap mx, mw, mo;
+  if (!make_map(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a->hidden, a->n_rows, a->hidden_dim, a->hidden_stride, kBM) ||
+      !make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a->weight, a->vocab, a->hidden_dim, a->weight_stride, Tile<BN, CTAS>::kBRows))
     return MLLM_GRPO_ERR_NO_DEVICE;
-  int64_t grid;
+  mo = mx;  // not read unless the output goes out by TMA
+  if (!STATS && p.out_aligned) {
+    const CUtensorMapDataType type = sizeof(O) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    if (!make_map(&mo, type, int(sizeof(O)), p.out, p.n_rows, p.vocab, p.out_stride * int64_t(sizeof(O)), 32))
+      return MLLM_GRPO_ERR_NO_DEVICE;
+  }
+  const int64_t m_teams = (p.m_tiles + CTAS - 1) / CTAS;
+  int64_t teams;
   if (STATS) {
     fold_plan(p.n_rows, p.vocab, &p.tiles_per_split, &p.splits);
-    grid = int64_t(p.m_tiles) * p.splits;
+    teams = m_teams * p.splits;
   } else {
-    grid = int64_t(p.m_tiles) * p.n_tiles;
-    if (grid >= (int64_t(1) << 30)) return MLLM_GRPO_ERR_TOO_LARGE;
-    if (grid > kSms) grid = kSms;
+    teams = m_teams * p.n_tiles;
   }
-  if (grid >= (int64_t(1) << 30)) return MLLM_GRPO_ERR_TOO_LARGE;
-  return launch_t<BN, STATS, O>(p, unsigned(grid), mx, mw, s);
+  if (teams >= (int64_t(1) << 29)) return MLLM_GRPO_ERR_TOO_LARGE;
+  if (!STATS && teams > kSms / CTAS) teams = kSms / CTAS;
+  return launch_t<BN, CTAS, STATS, O>(p, unsigned(teams * CTAS), mx, mw, mo, s);
 }
 
 template <typename O>
 static int launch_product(const Params& p, const mllm_lm_head_fp8_args* a, cudaStream_t s) {
   // tiles of 256 columns read the least per product; with fewer of them than SMs, twice as many of 128
-  const int64_t tiles = ((p.n_rows + kBM - 1) / kBM) * ((p.vocab + 255) / 256);
-  return tiles <= kSms ? launch<128, false, O>(p, a, s) : launch<256, false, O>(p, a, s);
+  const int64_t m_tiles = (p.n_rows + kBM - 1) / kBM, tiles = m_tiles * ((p.vocab + 255) / 256);
+  if (tiles <= kSms) return launch<128, 1, false, O>(p, a, s);
+  return ctas_for(m_tiles) == 2 ? launch<256, 2, false, O>(p, a, s) : launch<256, 1, false, O>(p, a, s);
 }
 
 static bool aligned(const void* q, uintptr_t a) { return (reinterpret_cast<uintptr_t>(q) & (a - 1)) == 0; }
@@ -550,7 +797,8 @@ int mllm_lm_head_fp8_partials(const mllm_lm_head_fp8_args* a, void* stream) {
   p.vocab_start = a->vocab_start;
   p.vocab_total = a->vocab_total > 0 ? a->vocab_total : a->vocab_start + a->vocab;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = fp8::launch<fp8::kFoldBN, true, float>(p, a, s);
+  st = fp8::ctas_for((a->n_rows + fp8::kBM - 1) / fp8::kBM) == 2 ? fp8::launch<fp8::kFoldBN, 2, true, float>(p, a, s)
+                                                                  : fp8::launch<fp8::kFoldBN, 1, true, float>(p, a, s);
   if (st) return st;
   int per, splits;
   fp8::fold_plan(a->n_rows, a->vocab, &per, &splits);

@@ -91,7 +91,7 @@ def _operands(M, N, K, seed, dev):
 SHAPES = [
     (1, 1, 16), (1, 128, 128), (1, 1000, 896), (2, 4099, 272), (7, 300, 3584), (8, 129, 64), (9, 640, 1040), (16, 2048, 512),
     (17, 257, 384), (33, 513, 160), (64, 1024, 2048), (128, 256, 128), (129, 255, 144), (300, 1111, 400), (257, 4096, 1792),
-    (1000, 20000, 256),
+    (1000, 20000, 256), (257, 19001, 144), (300, 30000, 16), (128, 40000, 400), (140, 38000, 1056),
 ]
 
 
