@@ -773,6 +773,10 @@ int mllm_lm_head_fp8_matmul(const mllm_lm_head_fp8_args* a, void* stream) {
   if (!fp8::aligned(a->out, es)) return MLLM_GRPO_ERR_ALIGNMENT;
   p.out_aligned = fp8::aligned(a->out, 16) && (a->out_stride * es) % 16 == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->n_rows <= fp8::kFewRows) {
+    const cudaError_t e = fp8::launch_few_rows(p, a->out_dtype, s);
+    return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);
+  }
   if (a->out_dtype == MLLM_GRPO_F32) return fp8::launch_product<float>(p, a, s);
   if (a->out_dtype == MLLM_GRPO_F16) return fp8::launch_product<__half>(p, a, s);
   return fp8::launch_product<__nv_bfloat16>(p, a, s);
