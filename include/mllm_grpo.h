@@ -418,7 +418,7 @@ int mllm_grpo_embedding_lookup(const mllm_grpo_embedding_args* args, void* strea
 /* dweight[v, :] = scale * sum over n with ids[n] == v of grad_out[n, :]: the tokens are sorted by id first (stable,
  * one launch), so every row is summed in f32 in an order that depends on the ids alone; no floating-point atomics. */
 int mllm_grpo_embedding_grad(const mllm_grpo_embedding_args* args, void* stream);
-int64_t mllm_grpo_embedding_workspace_bytes(int64_t n_tokens, int64_t hidden);
+int64_t mllm_grpo_embedding_workspace_bytes(int64_t n_tokens, int64_t hidden, int64_t vocab);
 
 /* ---- 8-bit floating point (e4m3) with a scale for each block of 128 ----
  * scale = max(amax, 448 * 2^-126) / 448 over a block of block_rows x 128 elements, q = e4m3(448 x / amax) to nearest

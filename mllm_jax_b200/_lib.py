@@ -183,8 +183,9 @@ def load():
         fn = getattr(lib, name)
         fn.argtypes = [C.POINTER(args), C.c_void_p]
         fn.restype = C.c_int
-    for name in ("mllm_grpo_preference_workspace_bytes", "mllm_grpo_embedding_workspace_bytes",
-                 "mllm_lm_head_fp8_partials_bytes"):
+    lib.mllm_grpo_embedding_workspace_bytes.argtypes = [C.c_int64] * 3
+    lib.mllm_grpo_embedding_workspace_bytes.restype = C.c_int64
+    for name in ("mllm_grpo_preference_workspace_bytes", "mllm_lm_head_fp8_partials_bytes"):
         fn = getattr(lib, name)
         fn.argtypes = [C.c_int64, C.c_int64]
         fn.restype = C.c_int64

@@ -5,13 +5,18 @@
 // Lookup: N*H elements read and written, bound by memory; one thread moves one vector of a row.
 //
 // Gradient: the new [V, H] gradient has to be written whole (at V = 151936, H = 3584 that is 2.18 GB of f32 against
-// 0.23 GB of token gradients), so the kernel that writes it walks the TABLE's rows and sums a row's tokens on the
-// way.  It needs the tokens grouped by id in an order that depends on the ids alone: a stable radix sort of
-// (id, token) pairs by ONE cluster of eight CTAs, whose digit counts meet in distributed shared memory, in one
-// launch.  A row with very many tokens (padding, a frequent word) would keep one CTA busy long after all others:
-// runs of 32 equal ids that start at a multiple of 32 in the sorted order are summed beforehand, and runs of 1024
-// from those, so that a row of any length is a few dozen additions.  Every sum is f32 in a fixed order.
+// 0.23 GB of token gradients), nearly all of it zeros.  Its sums need the tokens grouped by id in an order that depends
+// on the ids alone: a stable radix sort of (id, token) pairs by ONE cluster of eight CTAs, whose digit counts meet in
+// distributed shared memory.  Then, in one launch, a few resident CTAs sum and write the rows that have tokens from a
+// list of them, and short CTAs fill the others with zeros, 32 KB each in the order of the addresses.  (CTAs that stay
+// resident and walk the table fill it at 6.1 TB/s, short ones in order at 7.5.  A loop over the table's rows that sums
+// where there are tokens holds the fill up: a load waits several microseconds behind the stores.)
+// A row with very many tokens (padding, a frequent word) would keep one CTA busy long after all others: runs of 32
+// equal ids that start at a multiple of 32 in the sorted order are summed beforehand, and eight warps share what is left
+// of such a row.  Every sum is f32 in a fixed order.
 #include <cuda_fp16.h>
+
+#include <cstring>
 
 #include "grpo_cluster.cuh"
 #include "grpo_common.cuh"
@@ -103,12 +108,13 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const LookupParams p) 
 }
 
 // ---------------------------------------------------------------------------------------------
-// Stable radix sort of (id, token) by one cluster of eight CTAs, 9 bits a pass.  CTA r owns the r-th eighth of
-// the pairs.  A pass: digit counts of the eighth; all eight counts through distributed shared memory give every
-// digit its first place; then tiles of 4096 pairs, 128 consecutive ones per warp, get their places by the warp's
-// match of equal digits (stable: lower lanes first) and the running counts of the warps before it.
+// Stable radix sort of (id, token) by one cluster of eight CTAs (one CTA for up to 4096 pairs), 9 bits a pass.  CTA r
+// owns the r-th eighth of the pairs, in tiles of 4096, 128 consecutive pairs per warp.  Inside a tile a pair's place among
+// its digit is found by the warp's match of equal digits (stable: lower lanes first) and the running counts of the warps
+// before it; all eight CTAs' digit counts through distributed shared memory give every digit its first place.  Two
+// passes: 12 us for up to 4096 pairs, 25 us for 32768.
 // ---------------------------------------------------------------------------------------------
-constexpr int kSortCtas = 8;
+constexpr int kSortCtas = 8;      // of a cluster, for more than one tile
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kRounds = 4;
@@ -123,6 +129,8 @@ struct SortParams {
   const int32_t* ids;
   uint32_t* key[2];  // ping-pong; the result is in key[(passes - 1) & 1]
   uint32_t* idx[2];
+  uint4* busy;       // 16 rows' marks a word, to be zeroed by the CTAs behind the sort's (none for an accumulated gradient)
+  uint32_t* counts;  // [2] to be zeroed
   int32_t* device_status;
 };
 
@@ -132,45 +140,116 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   return v;
 }
 
-__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) {
+template <int CTAS>
+__device__ __forceinline__ void sort_sync() {
+  if (CTAS == 1)
+    __syncthreads();
+  else
+    cl::cluster_sync_all();
+}
+
+template <int CTAS>
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) {
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t first[kBins];
-  __shared__ uint16_t count[kSortWarps][kBins];
+  __shared__ alignas(16) uint16_t count[kSortWarps][kBins];
   __shared__ uint32_t scan[kBins / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t rank = cl::cluster_rank();
-  const uint32_t per = (p.n + kSortCtas - 1) / kSortCtas;
+  if (blockIdx.x >= CTAS) {  // whole clusters
+    const int64_t words = (p.vocab + 15) / 16, step = int64_t(gridDim.x - CTAS) * kSortThreads;
+    for (int64_t i = int64_t(blockIdx.x - CTAS) * kSortThreads + tid; i < words; i += step) p.busy[i] = make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
+  const uint32_t rank = CTAS == 1 ? 0u : cl::cluster_rank();
+  const uint32_t per = (p.n + CTAS - 1) / CTAS;
   const uint32_t lo = min(p.n, rank * per), hi = min(p.n, lo + per);
   const uint32_t lower = (1u << lane) - 1u;
+  const bool one_tile = CTAS == 1 || per <= uint32_t(kTile);  // then the tile's counts are the eighth's
+  if (rank == 0 && tid < 2) p.counts[tid] = 0u;
 
   for (int pass = 0; pass < p.passes; ++pass) {
     const int shift = pass * kBits;
+    const bool odd = pass & 1;
+    const uint32_t* key_in = odd ? p.key[0] : p.key[1];
+    const uint32_t* idx_in = odd ? p.idx[0] : p.idx[1];
+    uint32_t* key_out = odd ? p.key[1] : p.key[0];
+    uint32_t* idx_out = odd ? p.idx[1] : p.idx[0];
     auto key_of = [&](uint32_t i) -> uint32_t {
-      if (pass) return __ldcg(p.key[(pass - 1) & 1] + i);
+      if (pass) return __ldcg(key_in + i);
       const int64_t id = p.ids[i], local = id - p.vocab_start;
       if (local >= 0 && local < p.vocab) return uint32_t(local);
+      if ((id < 0 || id >= p.vocab_total) && p.device_status) atomicOr(p.device_status, MLLM_GRPO_DEV_ID_IGNORED);
       return uint32_t(p.vocab);  // no row of this table: sorted behind all others
     };
-    for (int b = tid; b < kBins; b += kSortThreads) hist[b] = 0;
-    __syncthreads();
-    for (uint32_t i0 = lo; i0 < hi; i0 += kSortThreads) {
-      const uint32_t i = i0 + tid;
-      const bool ok = i < hi;
-      const uint32_t k = ok ? key_of(i) : 0u;
-      if (pass == 0 && ok && p.device_status) {
-        const int64_t id = p.ids[i];
-        if (id < 0 || id >= p.vocab_total) atomicOr(p.device_status, MLLM_GRPO_DEV_ID_IGNORED);
+    // one tile: keys, tokens, and the places among their digits; leaves the digits' totals of a thread's bin
+    uint32_t k[kRounds], n[kRounds], place[kRounds];
+    auto rank_tile = [&](uint32_t t0) -> uint32_t {
+      uint4* z = reinterpret_cast<uint4*>(&count[0][0]);
+      for (int i = tid; i < int(sizeof(count) / 16); i += kSortThreads) z[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        const uint32_t i = t0 + uint32_t(warp * (32 * kRounds) + r * 32 + lane);
+        const bool ok = i < hi;
+        k[r] = ok ? key_of(i) : 0u;
+        n[r] = ok ? (pass ? __ldcg(idx_in + i) : i) : 0xffffffffu;
       }
-      const uint32_t d = ok ? (k >> shift) & (kBins - 1) : uint32_t(kBins);
-      const uint32_t same = __match_any_sync(0xffffffffu, d);
-      if (ok && (same & lower) == 0) atomicAdd(&hist[d], __popc(same));
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        const bool ok = n[r] != 0xffffffffu;
+        const uint32_t d = ok ? (k[r] >> shift) & (kBins - 1) : uint32_t(kBins);
+        const uint32_t same = __match_any_sync(0xffffffffu, d);
+        place[r] = ok ? count[warp][d] + __popc(same & lower) : 0u;
+        __syncwarp();
+        if (ok && (same & lower) == 0) count[warp][d] = uint16_t(count[warp][d] + __popc(same));
+        __syncwarp();
+      }
+      __syncthreads();
+      uint32_t total = 0;
+      if (tid < kBins) {
+#pragma unroll 8
+        for (int w = 0; w < kSortWarps; ++w) {
+          const uint32_t c = count[w][tid];
+          count[w][tid] = uint16_t(total);
+          total += c;
+        }
+      }
+      return total;
+    };
+    auto scatter_tile = [&] {
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        if (n[r] == 0xffffffffu) continue;
+        const uint32_t d = (k[r] >> shift) & (kBins - 1);
+        const uint32_t to = first[d] + count[warp][d] + place[r];
+        key_out[to] = k[r];
+        idx_out[to] = n[r];
+      }
+    };
+
+    uint32_t tile_total = 0;
+    if (one_tile) {
+      tile_total = rank_tile(lo);
+      if (tid < kBins) hist[tid] = tile_total;
+    } else {
+      for (int b = tid; b < kBins; b += kSortThreads) hist[b] = 0;
+      __syncthreads();
+      for (uint32_t i0 = lo; i0 < hi; i0 += kSortThreads) {
+        const uint32_t i = i0 + tid;
+        const bool ok = i < hi;
+        const uint32_t d = ok ? (key_of(i) >> shift) & (kBins - 1) : uint32_t(kBins);
+        const uint32_t same = __match_any_sync(0xffffffffu, d);
+        if (ok && (same & lower) == 0) atomicAdd(&hist[d], __popc(same));
+      }
     }
-    cl::cluster_sync_all();
+    sort_sync<CTAS>();
     uint32_t total = 0, before = 0;
-    if (tid < kBins) {
+    if (CTAS == 1) {
+      total = tile_total;
+    } else if (tid < kBins) {
       const uint32_t mine = cl::smem_u32(&hist[tid]);
 #pragma unroll
-      for (int c = 0; c < kSortCtas; ++c) {
+      for (int c = 0; c < CTAS; ++c) {
         const uint32_t h = ld_cluster_u32(cl::map_to_cta(mine, c));
         total += h;
         if (c < int(rank)) before += h;
@@ -190,142 +269,148 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
       for (int w = 0; w < warp; ++w) base += scan[w];
       first[tid] = base;
     }
-    uint32_t* key_out = p.key[pass & 1];
-    uint32_t* idx_out = p.idx[pass & 1];
-    for (uint32_t t0 = lo; t0 < hi; t0 += kTile) {
-      uint4* z = reinterpret_cast<uint4*>(&count[0][0]);
-      for (int i = tid; i < int(sizeof(count) / 16); i += kSortThreads) z[i] = make_uint4(0, 0, 0, 0);
-      __syncthreads();
-      uint32_t k[kRounds], n[kRounds], place[kRounds];
-#pragma unroll
-      for (int r = 0; r < kRounds; ++r) {
-        const uint32_t i = t0 + uint32_t(warp * (32 * kRounds) + r * 32 + lane);
-        const bool ok = i < hi;
-        k[r] = ok ? key_of(i) : 0u;
-        n[r] = ok ? (pass ? __ldcg(p.idx[(pass - 1) & 1] + i) : i) : 0xffffffffu;
+    __syncthreads();
+    if (one_tile) {
+      scatter_tile();
+    } else {
+      for (uint32_t t0 = lo; t0 < hi; t0 += kTile) {
+        tile_total = rank_tile(t0);
+        __syncthreads();
+        scatter_tile();
+        __syncthreads();
+        if (tid < kBins) first[tid] += tile_total;
       }
-#pragma unroll
-      for (int r = 0; r < kRounds; ++r) {
-        const bool ok = n[r] != 0xffffffffu;
-        const uint32_t d = ok ? (k[r] >> shift) & (kBins - 1) : uint32_t(kBins);
-        const uint32_t same = __match_any_sync(0xffffffffu, d);
-        place[r] = ok ? count[warp][d] + __popc(same & lower) : 0u;
-        __syncwarp();
-        if (ok && (same & lower) == 0) count[warp][d] = uint16_t(count[warp][d] + __popc(same));
-        __syncwarp();
-      }
-      __syncthreads();
-      uint32_t tile_total = 0;
-      if (tid < kBins) {
-#pragma unroll 8
-        for (int w = 0; w < kSortWarps; ++w) {
-          const uint32_t c = count[w][tid];
-          count[w][tid] = uint16_t(tile_total);
-          tile_total += c;
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int r = 0; r < kRounds; ++r) {
-        if (n[r] == 0xffffffffu) continue;
-        const uint32_t d = (k[r] >> shift) & (kBins - 1);
-        const uint32_t to = first[d] + count[warp][d] + place[r];
-        key_out[to] = k[r];
-        idx_out[to] = n[r];
-      }
-      __syncthreads();
-      if (tid < kBins) first[tid] += tile_total;
     }
-    cl::cluster_sync_all();  // the pass's pairs are visible to the cluster, and nobody reads `hist` any more
+    sort_sync<CTAS>();  // the pass's pairs are visible to the cluster, and nobody reads `hist` any more
   }
 }
 
 // ---------------------------------------------------------------------------------------------
 // Sums
 // ---------------------------------------------------------------------------------------------
-constexpr int kRun = 32, kSuper = 1024;
+constexpr uint32_t kRun = 32;
+constexpr int kSumWarps = kThreads / 32;
+constexpr int kCols = 4;  // vectors of a light row that a thread has on the way
+
+// The rows that have tokens, in no particular order (each is summed by itself): light ones with up to kLight tokens,
+// whose records say all that is needed to start, and heavy ones by the place of their first token.
+constexpr uint32_t kLight = 16;
+static_assert(kLight <= kRun, "");
+struct alignas(16) Light {
+  uint32_t row, first, count, pad;  // row of the table, sorted place of its first token, how many
+};
+struct Lists {
+  uint32_t* counts;  // [0] light rows, [1] heavy rows
+  Light* light;      // [n]
+  uint32_t* heavy;   // [n / (kLight + 1)]
+};
 
 struct GradParams {
-  int64_t vocab, grad_stride, weight_stride;
-  uint32_t n, hidden, row_vecs, rows_per_cta;
-  FastDiv by_row;
+  int64_t grad_stride, weight_stride;
+  uint32_t n, hidden, vocab, row_vecs, accumulate;
+  uint32_t group;  // threads that share a light row: 32, 64, 128 or 256
+  uint32_t parts;  // parts of 32 vectors of a row
+  uint32_t row_ctas;
+  FastDiv by_part;
   float scale;
   const uint32_t* key;
   const uint32_t* idx;
+  uint8_t* busy;  // [vocab] 1 where a row has tokens
+  Lists lists;
   const void* grad;
   void* dweight;
-  float* run;    // [n / 32, hidden]
-  float* super;  // [n / 1024, hidden]
+  float* run;  // [n / 32, hidden]
 };
 
 template <typename T, int EV>
-__device__ __forceinline__ void add_token(const GradParams& p, float (&acc)[EV], uint32_t token, uint32_t col) {
-  const Vec<T, EV> x = *(reinterpret_cast<const Vec<T, EV>*>(static_cast<const T*>(p.grad) + int64_t(token) * p.grad_stride) + col);
+__device__ __forceinline__ Vec<T, EV> token_vec(const GradParams& p, uint32_t token, uint32_t col) {
+  return *(reinterpret_cast<const Vec<T, EV>*>(static_cast<const T*>(p.grad) + int64_t(token) * p.grad_stride) + col);
+}
+template <typename T, int EV>
+__device__ __forceinline__ void add_vec(float (&acc)[EV], const Vec<T, EV>& x) {
 #pragma unroll
   for (int j = 0; j < EV; ++j) acc[j] += Conv<T>::up(x.v[j]);
 }
+// f32 sums are kept in rows of `hidden`, read and written four at a time where the width allows it (EV >= 4 does).
 template <int EV>
 __device__ __forceinline__ void add_sum(const GradParams& p, float (&acc)[EV], const float* sums, uint32_t row, uint32_t col) {
   const float* s = sums + int64_t(row) * p.hidden + int64_t(col) * EV;
+  if constexpr (EV >= 4) {
 #pragma unroll
-  for (int j = 0; j < EV; ++j) acc[j] += s[j];
-}
-
-// Runs of 32 equal ids.  blockIdx.x = run, blockIdx.y = part of the columns.
-template <typename T, int EV>
-__global__ void __launch_bounds__(kThreads) run_kernel(const GradParams p) {
-  const uint32_t i0 = blockIdx.x * kRun;
-  const uint32_t k = p.key[i0];
-  if (k != p.key[i0 + kRun - 1] || k >= p.vocab) return;
-  for (uint32_t c = blockIdx.y * kThreads + threadIdx.x; c < p.row_vecs; c += gridDim.y * kThreads) {
-    float acc[EV] = {};
-#pragma unroll 8
-    for (int i = 0; i < kRun; ++i) add_token<T, EV>(p, acc, p.idx[i0 + i], c);
-    float* out = p.run + int64_t(blockIdx.x) * p.hidden + int64_t(c) * EV;
-#pragma unroll
-    for (int j = 0; j < EV; ++j) out[j] = acc[j];
-  }
-}
-template <int EV>
-__global__ void __launch_bounds__(kThreads) super_kernel(const GradParams p) {
-  const uint32_t i0 = blockIdx.x * kSuper;
-  const uint32_t k = p.key[i0];
-  if (k != p.key[i0 + kSuper - 1] || k >= p.vocab) return;
-  for (uint32_t c = blockIdx.y * kThreads + threadIdx.x; c < p.row_vecs; c += gridDim.y * kThreads) {
-    float acc[EV] = {};
-#pragma unroll 8
-    for (int i = 0; i < kSuper / kRun; ++i) add_sum<EV>(p, acc, p.run, blockIdx.x * (kSuper / kRun) + i, c);
-    float* out = p.super + int64_t(blockIdx.x) * p.hidden + int64_t(c) * EV;
-#pragma unroll
-    for (int j = 0; j < EV; ++j) out[j] = acc[j];
-  }
-}
-
-// Sum of the tokens at sorted places [s, e) in one vector of columns.
-template <typename T, int EV>
-__device__ __forceinline__ void segment_sum(const GradParams& p, float (&acc)[EV], uint32_t s, uint32_t e, uint32_t col) {
-  uint32_t i = s;
-  while (i < e) {
-    if ((i & (kSuper - 1)) == 0 && i + kSuper <= e) {
-      const uint32_t n = (e - i) / kSuper;
-#pragma unroll 4
-      for (uint32_t q = 0; q < n; ++q) add_sum<EV>(p, acc, p.super, i / kSuper + q, col);
-      i += n * kSuper;
-    } else if ((i & (kRun - 1)) == 0 && i + kRun <= e) {
-      // up to the next multiple of 1024 (or the end)
-      const uint32_t stop = min(e, (i & ~uint32_t(kSuper - 1)) + kSuper);
-      const uint32_t n = (stop - i) / kRun;
-#pragma unroll 4
-      for (uint32_t q = 0; q < n; ++q) add_sum<EV>(p, acc, p.run, i / kRun + q, col);
-      i += n * kRun;
-    } else {
-      const uint32_t stop = min(e, (i & ~uint32_t(kRun - 1)) + kRun);
-#pragma unroll 4
-      for (; i < stop; ++i) add_token<T, EV>(p, acc, p.idx[i], col);
+    for (int j = 0; j < EV; j += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(s + j);
+      acc[j] += v.x;
+      acc[j + 1] += v.y;
+      acc[j + 2] += v.z;
+      acc[j + 3] += v.w;
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < EV; ++j) acc[j] += s[j];
+  }
+}
+template <typename O, int EV>
+__device__ __forceinline__ void store_vec(O* to, const float (&acc)[EV], float scale) {
+  constexpr int kPart = EV * int(sizeof(O)) > 16 ? 16 / int(sizeof(O)) : EV;
+#pragma unroll
+  for (int i = 0; i < EV; i += kPart) {
+    Vec<O, kPart> y;
+#pragma unroll
+    for (int j = 0; j < kPart; ++j) y.v[j] = Conv<O>::down(acc[i + j] * scale);
+    *reinterpret_cast<Vec<O, kPart>*>(to + i) = y;
   }
 }
 
+// Lists and marks the rows that have tokens (CTAs of their own), and sums runs of 32 equal ids, 8 token rows of 16
+// bytes a thread (16 of 8 or fewer) on the way at a time.  blockIdx.x = 32 sorted places, blockIdx.y = part of the columns.
+template <typename T, int EV>
+__global__ void __launch_bounds__(128) run_kernel(const GradParams p, const uint32_t row_vecs) {
+  constexpr uint32_t B = EV * sizeof(T) == 16 ? 8 : 16;
+  const uint32_t lane = threadIdx.x & 31, i = blockIdx.x * kRun + lane;
+  const uint32_t mine = i < p.n ? p.key[i] : 0xffffffffu;
+  const uint32_t tokens = i < p.n ? p.idx[i] : 0u;
+  if (blockIdx.y == gridDim.y - 1) {  // the last one has no columns: it lists and marks
+    if (threadIdx.x >= 32) return;
+    const uint32_t before = i > 0 && i < p.n ? p.key[i - 1] : 0xffffffffu;
+    const uint32_t after = i + kRun < p.n ? p.key[i + kRun] : 0xffffffffu;  // the next 32 places
+    const bool head = mine < p.vocab && (i == 0 || before != mine);
+    // how many tokens the row has (up to 64 are seen from here): equal keys are neighbours
+    const uint32_t last = __shfl_sync(0xffffffffu, mine, 31);
+    const uint32_t over = __popc(__ballot_sync(0xffffffffu, after == last));
+    const uint32_t count = __popc(__match_any_sync(0xffffffffu, mine)) + (mine == last ? over : 0u);
+    const bool heavy = head && count > kLight;
+    const uint32_t lower = (1u << lane) - 1u;
+    const uint32_t hs = __ballot_sync(0xffffffffu, heavy), ls = __ballot_sync(0xffffffffu, head && !heavy);
+    uint32_t at = 0;
+    if (lane == 0 && ls) at = atomicAdd(p.lists.counts, uint32_t(__popc(ls)));
+    if (lane == 1 && hs) at = atomicAdd(p.lists.counts + 1, uint32_t(__popc(hs)));
+    const uint32_t lb = __shfl_sync(0xffffffffu, at, 0), hb = __shfl_sync(0xffffffffu, at, 1);
+    if (heavy)
+      p.lists.heavy[hb + __popc(hs & lower)] = i;
+    else if (head)
+      p.lists.light[lb + __popc(ls & lower)] = Light{mine, i, count, 0u};
+    if (head && !p.accumulate) p.busy[mine] = 1;
+    return;
+  }
+  const uint32_t k = __shfl_sync(0xffffffffu, mine, 0);
+  if (__shfl_sync(0xffffffffu, mine, 31) != k || k >= p.vocab) return;
+  const uint32_t c = blockIdx.y * 128 + threadIdx.x;
+  const bool ok = c < row_vecs;
+  float acc[EV] = {};
+#pragma unroll
+  for (uint32_t q = 0; q < kRun; q += B) {
+    Vec<T, EV> x[B];
+#pragma unroll
+    for (uint32_t j = 0; j < B; ++j) {
+      const uint32_t token = __shfl_sync(0xffffffffu, tokens, q + j);
+      if (ok) x[j] = token_vec<T, EV>(p, token, c);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < B; ++j)
+      if (ok) add_vec<T, EV>(acc, x[j]);
+  }
+  if (ok) store_vec<float, EV>(p.run + int64_t(blockIdx.x) * p.hidden + int64_t(c) * EV, acc, 1.0f);
+}
 // First place in [lo, hi) whose key is >= v, found by a whole warp (32 probes a step).
 __device__ __forceinline__ uint32_t warp_lower_bound(const uint32_t* key, uint32_t lo, uint32_t hi, uint64_t v) {
   const uint32_t lane = threadIdx.x & 31;
@@ -344,70 +429,142 @@ __device__ __forceinline__ uint32_t warp_lower_bound(const uint32_t* key, uint32
 }
 
 template <typename O, int EV>
-__device__ __forceinline__ void store_row(O* to, const float (&acc)[EV], float scale) {
-  Vec<O, EV> y;
+__device__ __forceinline__ void finish_row(const GradParams& p, const float (&acc)[EV], uint32_t row, uint32_t col) {
+  O* to = static_cast<O*>(p.dweight) + int64_t(row) * p.weight_stride + int64_t(col) * EV;
+  if (p.accumulate) {
 #pragma unroll
-  for (int j = 0; j < EV; ++j) y.v[j] = Conv<O>::down(acc[j] * scale);
-  *reinterpret_cast<Vec<O, EV>*>(to) = y;
+    for (int j = 0; j < EV; ++j) to[j] = Conv<O>::down(Conv<O>::up(to[j]) + acc[j] * p.scale);
+  } else {
+    store_vec<O, EV>(to, acc, p.scale);
+  }
 }
 
-constexpr int kMostRows = kThreads;
-
-// Writes rows_per_cta consecutive rows of the table's gradient: zeros, or the sum of the row's tokens.
+// Rows with more than kLight tokens, 32 vectors of one per CTA and step: its single tokens and its runs go round the
+// eight warps, which meet in shared memory.
 template <typename T, typename O, int EV>
-__global__ void __launch_bounds__(kThreads) dense_grad_kernel(const GradParams p) {
-  __shared__ uint32_t bound[2];
-  __shared__ uint32_t at[kMostRows + 1];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t v0 = int64_t(blockIdx.x) * p.rows_per_cta;
-  const uint32_t rows = uint32_t(p.vocab - v0 < p.rows_per_cta ? p.vocab - v0 : p.rows_per_cta);
-  if (warp < 2) {
-    const uint32_t b = warp_lower_bound(p.key, 0, p.n, uint64_t(v0) + (warp ? rows : 0));
-    if (lane == 0) bound[warp] = b;
-  }
-  __syncthreads();
-  const uint32_t s = bound[0], e = bound[1];
-  for (uint32_t r = tid; r <= rows; r += kThreads) {
-    uint32_t lo = s, hi = e;
-    const uint32_t v = uint32_t(v0) + r;
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (p.key[mid] < v)
-        lo = mid + 1;
-      else
-        hi = mid;
-    }
-    at[r] = lo;
-  }
-  __syncthreads();
-  O* out = static_cast<O*>(p.dweight) + v0 * p.weight_stride;
-  const uint32_t items = rows * p.row_vecs;
-  for (uint32_t i = tid; i < items; i += kThreads) {
-    const uint32_t r = p.by_row.div(i), c = i - r * p.row_vecs;
+__device__ __forceinline__ void heavy_rows(const GradParams& p, float (&meet)[kSumWarps][32][EV]) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t items = p.lists.counts[1] * p.parts;
+  for (uint32_t item = blockIdx.x; item < items; item += p.row_ctas) {
+    const uint32_t r = p.by_part.div(item), c = (item - r * p.parts) * 32 + lane;
+    const bool ok = c < p.row_vecs;
+    const uint32_t s = p.lists.heavy[r], k = p.key[s];
+    const uint32_t e = warp_lower_bound(p.key, s + kLight, p.n, uint64_t(k) + 1);
+    // single tokens up to a multiple of 32, whole runs, the tokens behind the last of them
+    const uint32_t a0 = min(e, (s + kRun - 1) / kRun * kRun), a1 = max(a0, e / kRun * kRun);
     float acc[EV] = {};
-    const uint32_t a = at[r], b = at[r + 1];
-    if (a != b) segment_sum<T, EV>(p, acc, a, b, c);
-    store_row<O, EV>(out + int64_t(r) * p.weight_stride + int64_t(c) * EV, acc, p.scale);
+    if (ok) {
+#pragma unroll 4
+      for (uint32_t i = s + warp; i < a0; i += kSumWarps) add_vec<T, EV>(acc, token_vec<T, EV>(p, p.idx[i], c));
+#pragma unroll 4
+      for (uint32_t q = a0 / kRun + warp; q < a1 / kRun; q += kSumWarps) add_sum<EV>(p, acc, p.run, q, c);
+#pragma unroll 4
+      for (uint32_t i = a1 + warp; i < e; i += kSumWarps) add_vec<T, EV>(acc, token_vec<T, EV>(p, p.idx[i], c));
+    }
+#pragma unroll
+    for (int j = 0; j < EV; ++j) meet[warp][lane][j] = acc[j];
+    __syncthreads();
+    if (warp == 0 && ok) {
+#pragma unroll
+      for (int w = 1; w < kSumWarps; ++w)
+#pragma unroll
+        for (int j = 0; j < EV; ++j) acc[j] += meet[w][lane][j];
+      finish_row<O, EV>(p, acc, k, c);
+    }
+    __syncthreads();
   }
 }
 
-// Adds to the rows that have tokens.  One CTA per sorted place; the first of an id does the row.
-template <typename T, int EV>
-__global__ void __launch_bounds__(kThreads) accumulate_grad_kernel(const GradParams p) {
-  const uint32_t s = blockIdx.x;
-  const uint32_t k = p.key[s];
-  if (k >= p.vocab || (s > 0 && p.key[s - 1] == k)) return;
-  const uint32_t e = s + 1 < p.n && p.key[s + 1] == k ? warp_lower_bound(p.key, s + 1, p.n, uint64_t(k) + 1) : s + 1;
-  float* out = static_cast<float*>(p.dweight) + int64_t(k) * p.weight_stride;
-  for (uint32_t c = threadIdx.x; c < p.row_vecs; c += kThreads) {
-    float acc[EV] = {};
-    segment_sum<T, EV>(p, acc, s, e, c);
-    Vec<float, EV>* to = reinterpret_cast<Vec<float, EV>*>(out) + c;
-    Vec<float, EV> y = *to;
+// Rows with up to kLight tokens, p.group threads each, kCols vectors a thread.  While one is summed, the next one's
+// tokens and the record of the one after that are on their way.
+template <typename T, typename O, int EV>
+__device__ __forceinline__ void light_rows(const GradParams& p) {
+  const uint32_t lane = threadIdx.x & 31, groups = kThreads / p.group, mine = threadIdx.x / p.group, at = threadIdx.x % p.group;
+  const uint32_t rows = p.lists.counts[0], step = p.row_ctas * groups;
+  const Light none{0, 0, 0, 0};
+  auto record = [&](uint32_t r) { return r < rows ? p.lists.light[r] : none; };
+  auto tokens_of = [&](const Light& l) { return lane < l.count ? p.idx[l.first + lane] : 0u; };
+  uint32_t r = blockIdx.x * groups + mine;
+  Light now = record(r), next = record(r + step);
+  uint32_t tokens = tokens_of(now);
+  for (; r < rows; r += step) {
+    const Light after = record(r + 2 * step);
+    const uint32_t next_tokens = tokens_of(next);
+    for (uint32_t c0 = at; c0 < p.row_vecs + at; c0 += p.group * kCols) {  // whole warps: the tokens come from its lanes
+      float acc[kCols][EV] = {};
+      for (uint32_t i = 0; i < now.count; i += 2) {
+        Vec<T, EV> x[2][kCols];
+        const uint32_t first = __shfl_sync(0xffffffffu, tokens, i & 31), second = __shfl_sync(0xffffffffu, tokens, (i + 1) & 31);
+        const bool two = i + 1 < now.count;
 #pragma unroll
-    for (int j = 0; j < EV; ++j) y.v[j] += acc[j] * p.scale;
-    *to = y;
+        for (int u = 0; u < kCols; ++u) {
+          const uint32_t c = c0 + u * p.group;
+          if (c < p.row_vecs) x[0][u] = token_vec<T, EV>(p, first, c);
+          if (two && c < p.row_vecs) x[1][u] = token_vec<T, EV>(p, second, c);
+        }
+#pragma unroll
+        for (int u = 0; u < kCols; ++u) {
+          const uint32_t c = c0 + u * p.group;
+          if (c < p.row_vecs) add_vec<T, EV>(acc[u], x[0][u]);
+          if (two && c < p.row_vecs) add_vec<T, EV>(acc[u], x[1][u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kCols; ++u)
+        if (c0 + u * p.group < p.row_vecs) finish_row<O, EV>(p, acc[u], now.row, c0 + u * p.group);
+    }
+    now = next;
+    next = after;
+    tokens = next_tokens;
   }
+}
+
+// Zeros in the rows without tokens, kVecs words W a thread in the order of their addresses.
+constexpr int kVecs = 8;
+struct FillParams {
+  int64_t stride;  // of a row, in words
+  uint32_t total;  // words of this launch's rows
+  uint32_t row_words;
+  FastDiv by_row;
+  const uint8_t* busy;  // of this launch's rows; null: no row has tokens
+  void* out;
+};
+template <typename W>
+__device__ __forceinline__ void fill(const FillParams& p, uint32_t block) {
+  const uint32_t base = block * uint32_t(kThreads * kVecs) + threadIdx.x;
+  uint32_t skip = 0;
+  if (p.busy) {
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const uint32_t i = base + u * kThreads;
+      if (i < p.total && p.busy[p.by_row.div(i)]) skip |= 1u << u;
+    }
+  }
+  W zero;
+  memset(&zero, 0, sizeof(W));
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const uint32_t i = base + u * kThreads;
+    if (i >= p.total || (skip >> u & 1u)) continue;
+    const uint32_t r = p.by_row.div(i);
+    static_cast<W*>(p.out)[r * p.stride + (i - r * p.row_words)] = zero;
+  }
+}
+template <typename W>
+__global__ void __launch_bounds__(kThreads, 8) fill_kernel(const FillParams p) {
+  fill<W>(p, blockIdx.x);
+}
+
+// CTAs [0, p.row_ctas) sum the rows that have tokens; the others fill.
+template <typename T, typename O, int EV, typename W>
+__global__ void __launch_bounds__(kThreads, 4) grad_rows_kernel(const GradParams p, const FillParams f) {
+  __shared__ float meet[kSumWarps][32][EV];
+  if (blockIdx.x >= p.row_ctas) {
+    fill<W>(f, blockIdx.x - p.row_ctas);
+    return;
+  }
+  heavy_rows<T, O, EV>(p, meet);
+  light_rows<T, O, EV>(p);
 }
 
 static cudaError_t done() {
@@ -467,51 +624,112 @@ static cudaError_t launch_lookup_t(const mllm_grpo_embedding_args* a, LookupPara
 
 template <typename T, int EV>
 static cudaError_t launch_runs(const GradParams& p, cudaStream_t s) {
-  const unsigned ny = (p.row_vecs + kThreads - 1) / kThreads;
-  if (p.n >= kRun) {
-    run_kernel<T, EV><<<dim3(p.n / kRun, ny), kThreads, 0, s>>>(p);
-    const cudaError_t e = done();
-    if (e != cudaSuccess) return e;
-  }
-  if (p.n >= kSuper) {
-    super_kernel<EV><<<dim3(p.n / kSuper, ny), kThreads, 0, s>>>(p);
+  const uint32_t runs = (p.n + kRun - 1) / kRun;
+  const auto parts = [](uint32_t row_vecs) { return (row_vecs + 127) / 128 + 1; };
+  constexpr int kWide = 16 / int(sizeof(T));
+  if (vec_of(p.hidden, kWide, p.grad, p.grad_stride, sizeof(T), p.run, p.hidden, 2) == kWide)
+    run_kernel<T, kWide><<<dim3(runs, parts(p.hidden / kWide)), 128, 0, s>>>(p, p.hidden / kWide);
+  else
+    run_kernel<T, EV><<<dim3(runs, parts(p.row_vecs)), 128, 0, s>>>(p, p.row_vecs);
+  return done();
+}
+
+constexpr int64_t kMostWords = int64_t(1) << 31;  // words are counted in 32 bits
+
+// The rows [r0, r0 + rows) of the gradient in words of W.
+template <typename W>
+static FillParams fill_params(const mllm_grpo_embedding_args* a, const uint8_t* busy, int64_t r0, int64_t rows) {
+  const int64_t eo = elem(a->out_dtype), row_words = a->hidden * eo / int64_t(sizeof(W));
+  FillParams f{a->weight_stride * eo / int64_t(sizeof(W)), uint32_t(rows * row_words), uint32_t(row_words),
+               FastDiv(uint32_t(row_words)), busy ? busy + r0 : nullptr, nullptr};
+  f.out = static_cast<W*>(a->dweight) + r0 * f.stride;
+  return f;
+}
+static unsigned fill_ctas(const FillParams& f) { return (f.total + kThreads * kVecs - 1) / (kThreads * kVecs); }
+
+template <typename W>
+static cudaError_t launch_fill(const mllm_grpo_embedding_args* a, const uint8_t* busy, int64_t from, cudaStream_t s) {
+  const int64_t rows_per = kMostWords / (a->hidden * elem(a->out_dtype) / int64_t(sizeof(W)));
+  for (int64_t r0 = from; r0 < a->vocab; r0 += rows_per) {
+    const FillParams f = fill_params<W>(a, busy, r0, a->vocab - r0 < rows_per ? a->vocab - r0 : rows_per);
+    fill_kernel<W><<<fill_ctas(f), kThreads, 0, s>>>(f);
     const cudaError_t e = done();
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
 
+template <typename T, typename O, int EV, typename W>
+static cudaError_t launch_rows_w(const mllm_grpo_embedding_args* a, GradParams p, cudaStream_t s) {
+  // four CTAs are resident per SM: with many rows they are all busy with rows at first
+  const int64_t most = 148 * 4, items = (int64_t(p.n) * p.group + kThreads - 1) / kThreads;
+  p.row_ctas = uint32_t(items < most ? items : most);
+  if (a->accumulate) {
+    grad_rows_kernel<T, O, EV, W><<<p.row_ctas, kThreads, 0, s>>>(p, FillParams{0, 0, 1, FastDiv(1), nullptr, nullptr});
+    return done();
+  }
+  const int64_t rows_per = kMostWords / (a->hidden * elem(a->out_dtype) / int64_t(sizeof(W)));
+  const int64_t rows = a->vocab < rows_per ? a->vocab : rows_per;
+  const FillParams f = fill_params<W>(a, p.busy, 0, rows);
+  grad_rows_kernel<T, O, EV, W><<<p.row_ctas + fill_ctas(f), kThreads, 0, s>>>(p, f);
+  const cudaError_t e = done();
+  return e == cudaSuccess ? launch_fill<W>(a, p.busy, rows, s) : e;
+}
+
+// Zeros are written in the widest words that every row allows: 16 bytes, or an element.
+static bool wide_rows(const mllm_grpo_embedding_args* a) {
+  const int64_t eo = elem(a->out_dtype);
+  return ((a->hidden * eo | a->weight_stride * eo | int64_t(reinterpret_cast<uintptr_t>(a->dweight) & 15)) & 15) == 0;
+}
+
 template <typename T, typename O, int EV>
-static cudaError_t launch_dense(GradParams p, cudaStream_t s) {
-  // about 64 KB of gradient per CTA: enough to cover the search for the CTA's tokens
-  int64_t rows = 65536 / (int64_t(p.hidden) * int64_t(sizeof(O)));
-  rows = rows < 1 ? 1 : (rows > kMostRows ? kMostRows : rows);
-  p.rows_per_cta = uint32_t(rows);
-  dense_grad_kernel<T, O, EV><<<unsigned((p.vocab + rows - 1) / rows), kThreads, 0, s>>>(p);
-  return done();
+static cudaError_t launch_rows(const mllm_grpo_embedding_args* a, const GradParams& p, cudaStream_t s) {
+  if (wide_rows(a)) return launch_rows_w<T, O, EV, uint4>(a, p, s);
+  return launch_rows_w<T, O, EV, O>(a, p, s);
 }
 
 template <typename T, int EV>
 static cudaError_t launch_grad_ev(const mllm_grpo_embedding_args* a, const GradParams& p, cudaStream_t s) {
-  cudaError_t e = launch_runs<T, EV>(p, s);
+  const cudaError_t e = launch_runs<T, EV>(p, s);
   if (e != cudaSuccess) return e;
-  if (a->accumulate) {
-    if (p.n == 0) return cudaSuccess;
-    accumulate_grad_kernel<T, EV><<<p.n, kThreads, 0, s>>>(p);
-    return done();
-  }
-  if (a->out_dtype == MLLM_GRPO_F32) return launch_dense<T, float, EV>(p, s);
-  if (a->out_dtype == MLLM_GRPO_F16) return launch_dense<T, __half, EV>(p, s);
-  return launch_dense<T, __nv_bfloat16, EV>(p, s);
+  if (a->out_dtype == MLLM_GRPO_F32) return launch_rows<T, float, EV>(a, p, s);
+  if (a->out_dtype == MLLM_GRPO_F16) return launch_rows<T, __half, EV>(a, p, s);
+  return launch_rows<T, __nv_bfloat16, EV>(a, p, s);
 }
 
 template <typename T>
 static cudaError_t launch_grad_t(const mllm_grpo_embedding_args* a, GradParams p, cudaStream_t s) {
-  // four elements a vector: f32 rows are stored 16 bytes a thread
+  // four elements a vector (16 bytes of f32 sums and gradients), or one
   const int ev = vec_of(a->hidden, 4, a->grad_out, a->token_stride, sizeof(T), a->dweight, a->weight_stride, elem(a->out_dtype));
   p.row_vecs = uint32_t(a->hidden / (ev == 4 ? 4 : 1));
-  p.by_row = FastDiv(p.row_vecs);
+  p.group = 32;
+  while (p.group * kCols < p.row_vecs && p.group < uint32_t(kThreads)) p.group *= 2;
+  p.parts = (p.row_vecs + 31) / 32;
+  p.by_part = FastDiv(p.parts);
   return ev == 4 ? launch_grad_ev<T, 4>(a, p, s) : launch_grad_ev<T, 1>(a, p, s);
+}
+
+static cudaError_t launch_sort(const SortParams& q, bool zero_rows, cudaStream_t s) {
+  const bool small = q.n <= uint32_t(kTile);
+  // 16 rows' marks a thread, in whole clusters
+  int64_t more = zero_rows ? (q.vocab + kSortThreads * 16 - 1) / (kSortThreads * 16) : 0;
+  more = more > 128 ? 128 : more;
+  const int ctas = small ? 1 : kSortCtas;
+  more = (more + ctas - 1) / ctas * ctas;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(ctas + more));
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = unsigned(ctas);
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = small ? 0 : 1;
+  const cudaError_t e = small ? cudaLaunchKernelEx(&cfg, sort_kernel<1>, q) : cudaLaunchKernelEx(&cfg, sort_kernel<kSortCtas>, q);
+  count_launch();
+  return e;
 }
 
 static int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
@@ -559,9 +777,13 @@ int mllm_grpo_embedding_lookup(const mllm_grpo_embedding_args* a, void* stream) 
   return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);
 }
 
-int64_t mllm_grpo_embedding_workspace_bytes(int64_t n_tokens, int64_t hidden) {
-  if (n_tokens < 0 || hidden <= 0 || n_tokens >= (int64_t(1) << 31) || hidden > (int64_t(1) << 20)) return 0;
-  return 16 + 4 * emb::round16(n_tokens * 4) + (n_tokens / emb::kRun + n_tokens / emb::kSuper) * hidden * 4;
+int64_t mllm_grpo_embedding_workspace_bytes(int64_t n_tokens, int64_t hidden, int64_t vocab) {
+  if (n_tokens < 0 || hidden <= 0 || vocab <= 0 || n_tokens >= (int64_t(1) << 31) || hidden > (int64_t(1) << 20) ||
+      vocab >= (int64_t(1) << 31) - 1)
+    return 0;
+  // marks of the rows, two ping-pong pairs of lists, the lists of rows that have tokens, the sums of runs
+  return emb::round16(vocab) + 5 * emb::round16(n_tokens * 4) + 16 + n_tokens * int64_t(sizeof(emb::Light)) +
+         n_tokens / emb::kRun * hidden * 4;
 }
 
 int mllm_grpo_embedding_grad(const mllm_grpo_embedding_args* a, void* stream) {
@@ -575,6 +797,7 @@ int mllm_grpo_embedding_grad(const mllm_grpo_embedding_args* a, void* stream) {
     return MLLM_GRPO_ERR_ALIGNMENT;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const uint32_t n = uint32_t(a->n_tokens);
+  if (n == 0 && a->accumulate) return MLLM_GRPO_OK;
   char* w = static_cast<char*>(a->workspace);
   const int64_t list = emb::round16(int64_t(n) * 4);
   emb::SortParams q;
@@ -586,27 +809,43 @@ int mllm_grpo_embedding_grad(const mllm_grpo_embedding_args* a, void* stream) {
   while ((int64_t(1) << bits) <= a->vocab) ++bits;  // ids up to and including `vocab`, the mark of no row
   q.passes = (bits + emb::kBits - 1) / emb::kBits;
   q.ids = a->ids;
+  q.busy = reinterpret_cast<uint4*>(w);
+  w += emb::round16(a->vocab);
   for (int i = 0; i < 2; ++i) {
     q.key[i] = reinterpret_cast<uint32_t*>(w + (2 * i) * list);
     q.idx[i] = reinterpret_cast<uint32_t*>(w + (2 * i + 1) * list);
   }
+  w += 4 * list;
+  emb::Lists lists;
+  lists.heavy = reinterpret_cast<uint32_t*>(w);
+  lists.counts = reinterpret_cast<uint32_t*>(w + list);
+  lists.light = reinterpret_cast<emb::Light*>(w + list + 16);
+  q.counts = lists.counts;
   q.device_status = a->device_status;
+  const int last = (q.passes - 1) & 1;
   cudaError_t e = cudaSuccess;
   if (n) {
-    emb::sort_kernel<<<emb::kSortCtas, emb::kSortThreads, 0, s>>>(q);
-    e = emb::done();
+    e = emb::launch_sort(q, a->accumulate == 0, s);
     if (e != cudaSuccess) return record_cuda_error(e);
+    emb::GradParams p{a->token_stride, a->weight_stride, n, uint32_t(a->hidden), uint32_t(a->vocab), 0, a->accumulate ? 1u : 0u,
+                      0, 0, 0, emb::FastDiv(1), a->scale, q.key[last], q.idx[last], reinterpret_cast<uint8_t*>(q.busy), lists,
+                      a->grad_out, a->dweight,
+                      reinterpret_cast<float*>(w + list + 16 + int64_t(n) * int64_t(sizeof(emb::Light)))};
+    if (a->dtype == MLLM_GRPO_BF16)
+      e = emb::launch_grad_t<__nv_bfloat16>(a, p, s);
+    else if (a->dtype == MLLM_GRPO_F16)
+      e = emb::launch_grad_t<__half>(a, p, s);
+    else
+      e = emb::launch_grad_t<float>(a, p, s);
   }
-  const int last = (q.passes - 1) & 1;
-  float* run = reinterpret_cast<float*>(w + 4 * list);
-  emb::GradParams p{a->vocab, a->token_stride, a->weight_stride, n, uint32_t(a->hidden), 0, 0, emb::FastDiv(1), a->scale,
-                    q.key[last], q.idx[last], a->grad_out, a->dweight, run, run + int64_t(n / emb::kRun) * a->hidden};
-  if (a->dtype == MLLM_GRPO_BF16)
-    e = emb::launch_grad_t<__nv_bfloat16>(a, p, s);
-  else if (a->dtype == MLLM_GRPO_F16)
-    e = emb::launch_grad_t<__half>(a, p, s);
-  else
-    e = emb::launch_grad_t<float>(a, p, s);
+  if (n == 0) {  // all zeros (the accumulated form has returned)
+    if (emb::wide_rows(a))
+      e = emb::launch_fill<uint4>(a, nullptr, 0, s);
+    else if (a->out_dtype == MLLM_GRPO_F32)
+      e = emb::launch_fill<uint32_t>(a, nullptr, 0, s);
+    else
+      e = emb::launch_fill<uint16_t>(a, nullptr, 0, s);
+  }
   return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);
 }
 

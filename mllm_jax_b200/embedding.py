@@ -132,9 +132,9 @@ def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
         res = out
         a.weight_stride, a.out_dtype, a.accumulate = max(out.stride(0), H), _lib.DTYPE_F32, 1
     lib = _lib.load()
-    nbytes = int(lib.mllm_grpo_embedding_workspace_bytes(a.n_tokens, H))
+    nbytes = int(lib.mllm_grpo_embedding_workspace_bytes(a.n_tokens, H, vocab))
     if nbytes == 0:
-        raise ValueError(f"{a.n_tokens} tokens of {H} are too many for one call")
+        raise ValueError(f"{a.n_tokens} tokens, {vocab} rows of {H}: not a size that one call takes")
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     a.ids, a.grad_out, a.dweight, a.workspace = ids32.data_ptr(), g.data_ptr(), res.data_ptr(), workspace.data_ptr()
     _lib.launch("mllm_grpo_embedding_grad", a, dev)

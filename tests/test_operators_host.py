@@ -105,9 +105,11 @@ def test_embedding_entry_points_ask_for_what_they_read(built_lib):
     assert _status("mllm_grpo_embedding_grad", _emb(accumulate=1, out_dtype=0)) == 3
     assert _status("mllm_grpo_embedding_grad", _emb(out_dtype=4)) == 3
     assert _status("mllm_grpo_embedding_lookup", _emb(n_tokens=0, ids=None, weight=None, out=None)) == 0  # nothing to do
-    assert lib.mllm_grpo_embedding_workspace_bytes(-1, 8) == 0 and lib.mllm_grpo_embedding_workspace_bytes(5, 0) == 0
-    assert lib.mllm_grpo_embedding_workspace_bytes(0, 8) > 0
-    assert lib.mllm_grpo_embedding_workspace_bytes(4096, 100) >= 4 * 4096 * 4 + (128 + 4) * 100 * 4
+    for bad in ((-1, 8, 5), (5, 0, 5), (5, 8, 0), (1 << 31, 8, 5), (5, 8, 1 << 31)):
+        assert lib.mllm_grpo_embedding_workspace_bytes(*bad) == 0
+    assert lib.mllm_grpo_embedding_workspace_bytes(0, 8, 5) >= 5
+    # marks of 777 rows, four lists of tokens, a record per row that may have some, the sums of 128 runs
+    assert lib.mllm_grpo_embedding_workspace_bytes(4096, 100, 777) >= 777 + 4 * 4096 * 4 + 4096 * 16 + 128 * 100 * 4
 
 
 def _quant(**kw):
