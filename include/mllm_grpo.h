@@ -356,10 +356,13 @@ typedef struct mllm_grpo_preference_args {
   float grad_scale;      /* cotangent of the loss, used when grad_scale_dev is NULL */
   float total_pairs;     /* > 0; normaliser, used when total_pairs_dev is NULL */
   int32_t ref_per_sequence; /* 0: ref_logps is [2P*T]; 1: [2P], the reference's lp_s */
+  int64_t ids_stride;       /* elements between the sequences of chosen_ids; 0 = T (a slice of [2P, L] ids need not be copied) */
+  int64_t mask_stride;      /* likewise of mask */
+  int32_t mask_int;         /* 1: mask is int32 */
   const void* logits;       /* bf16 [2P, seq_rows, row_stride] */
-  const int32_t* chosen_ids;   /* [2P*T] */
+  const int32_t* chosen_ids;   /* [2P, T] */
   const float* token_logps;    /* [2P*T], mllm_grpo_preference_logps only */
-  const float* mask;           /* [2P*T] weights, or NULL = every scored row counts */
+  const void* mask;            /* [2P, T] weights, f32 or int32, or NULL = every scored row counts */
   const float* ref_logps;      /* or NULL */
   const float* pair_weights;   /* [P] or NULL */
   const float* total_pairs_dev;/* scalar in device memory or NULL */
@@ -371,7 +374,8 @@ typedef struct mllm_grpo_preference_args {
   void* dlogits;           /* bf16, may alias logits */
   void* workspace;         /* mllm_grpo_preference_workspace_bytes(...), 16-byte aligned; carries the residuals from
                               mllm_grpo_preference_fwd to mllm_grpo_preference_bwd */
-  int32_t* device_status;  /* optional */
+  int32_t* device_status;  /* optional: MLLM_GRPO_DEV_* bits are ORed in */
+  int32_t* call_status;    /* optional: set to this call's MLLM_GRPO_DEV_* bits (forward from logits) */
 } mllm_grpo_preference_args;
 
 /* Forward from logits: loss, rewards, sequence_logps and the residuals of the backward.  Rows with mask 0 are not read. */

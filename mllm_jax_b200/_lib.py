@@ -92,12 +92,12 @@ class PreferenceArgs(C.Structure):
         ("n_pairs", C.c_int64), ("seq_rows", C.c_int64), ("scored_rows", C.c_int64), ("vocab", C.c_int64),
         ("row_stride", C.c_int64), ("kind", C.c_int32), ("average", C.c_int32), ("beta", C.c_float),
         ("label_smoothing", C.c_float), ("softcap", C.c_float), ("grad_scale", C.c_float), ("total_pairs", C.c_float),
-        ("ref_per_sequence", C.c_int32),
+        ("ref_per_sequence", C.c_int32), ("ids_stride", C.c_int64), ("mask_stride", C.c_int64), ("mask_int", C.c_int32),
         ("logits", C.c_void_p), ("chosen_ids", C.c_void_p), ("token_logps", C.c_void_p), ("mask", C.c_void_p),
         ("ref_logps", C.c_void_p), ("pair_weights", C.c_void_p), ("total_pairs_dev", C.c_void_p),
         ("grad_scale_dev", C.c_void_p), ("loss", C.c_void_p), ("rewards", C.c_void_p), ("sequence_logps", C.c_void_p),
         ("dtoken_logps", C.c_void_p), ("dlogits", C.c_void_p), ("workspace", C.c_void_p),
-        ("device_status", C.c_void_p),
+        ("device_status", C.c_void_p), ("call_status", C.c_void_p),
     ]
 
 

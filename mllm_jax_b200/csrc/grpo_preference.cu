@@ -23,7 +23,7 @@ namespace pref {
 constexpr int kMaxSplits = 32;
 constexpr int64_t kTargetCtas = 592;    // 4 per SM
 constexpr int64_t kMinSplitCols = 8192; // 16 KB of a row per CTA at least
-constexpr int kPairThreads = 256;
+constexpr int kPairThreads = 512;
 constexpr int64_t kOneCtaTokens = 16384;
 
 struct Params {
@@ -34,7 +34,9 @@ struct Params {
   const uint16_t* logits;
   const int32_t* ids;
   const float* logps;
-  const float* mask;
+  const void* mask;
+  int64_t ids_stride, mask_stride;
+  int mask_int;
   const float* ref;
   const float* weights;
   const float* total_dev;
@@ -47,11 +49,12 @@ struct Params {
   // workspace
   double* terms;        // [P]
   float* coef;          // [2P]
-  unsigned int* ticket; // [1]
+  unsigned int* ticket; // [0] pairs done, [1] MLLM_GRPO_DEV_* bits of this call
   float* lse;           // [N]
   float* chosen;        // [N]
   float2* stats;        // [N, splits] (mk, S)
   int32_t* device_status;
+  int32_t* call_status;
 };
 
 __host__ __device__ inline int64_t round16(int64_t b) { return (b + 15) & ~int64_t(15); }
@@ -62,8 +65,12 @@ static int64_t max_splits(int64_t n_tokens) {
   return s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s);
 }
 
-__device__ __forceinline__ bool live_token(const Params& p, int64_t n, float* m) {
-  *m = p.mask ? p.mask[n] : 1.0f;
+__device__ __forceinline__ bool live_token(const Params& p, int64_t s, int64_t t, float* m) {
+  *m = 1.0f;
+  if (p.mask) {
+    const int64_t at = s * p.mask_stride + t;
+    *m = p.mask_int ? float(static_cast<const int32_t*>(p.mask)[at]) : static_cast<const float*>(p.mask)[at];
+  }
   return *m != 0.f;
 }
 
@@ -129,12 +136,12 @@ __global__ void __launch_bounds__(THREADS) pref_stats_kernel(const Params p) {
   constexpr int NW = THREADS / 32;
   __shared__ float red[2][NW];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (blockIdx.x == 0 && tid == 0) *p.ticket = 0u;
+  if (blockIdx.x == 0 && tid < 2) p.ticket[tid] = 0u;
   const int64_t n = blockIdx.x / unsigned(p.splits);
   const int k = int(blockIdx.x - n * p.splits);
   float mask;
-  if (!live_token(p, n, &mask)) return;
   const int64_t b = n / p.scored_rows, t = n - b * p.scored_rows;
+  if (!live_token(p, b, t, &mask)) return;
   const uint16_t* row = p.logits + (b * p.seq_rows + t) * p.row_stride;
   const int64_t c0 = int64_t(k) * p.split_cols;
   const int64_t V = p.vocab - c0 < p.split_cols ? p.vocab - c0 : p.split_cols;  // > 0 by the choice of splits
@@ -180,11 +187,8 @@ __global__ void __launch_bounds__(THREADS) pref_stats_kernel(const Params p) {
     const float S = warp_sum(lane < NW ? red[1][lane] * ex2f(m_in - M) : 0.f);
     if (lane == 0) {
       p.stats[n * p.splits + k] = make_float2(M, S);
-      int64_t c = p.ids[n];
-      if (c < 0 || c >= p.vocab) {
-        c = c < 0 ? 0 : p.vocab - 1;
-        if (p.device_status) atomicOr(p.device_status, MLLM_GRPO_DEV_ID_CLAMPED);
-      }
+      int64_t c = p.ids[b * p.ids_stride + t];
+      c = c < 0 ? 0 : (c >= p.vocab ? p.vocab - 1 : c);  // the launch that follows reports it
       if (c >= c0 && c < c0 + V) {
         const float x = __uint_as_float(uint32_t(row[c]) << 16);
         p.chosen[n] = CAP ? sc.y(x) : x;
@@ -193,10 +197,16 @@ __global__ void __launch_bounds__(THREADS) pref_stats_kernel(const Params p) {
   }
 }
 
-// Log-prob of token n in double precision; from logits, its log-sum-exp is kept for the backward sweep.
+// Log-prob of token (s, t) in double precision; from logits, its log-sum-exp is kept for the backward sweep.
 template <bool LOGPS>
-__device__ __forceinline__ double token_logp(const Params& p, int64_t n) {
+__device__ __forceinline__ double token_logp(const Params& p, int64_t s, int64_t t) {
+  const int64_t n = s * p.scored_rows + t;
   if (LOGPS) return double(p.logps[n]);
+  const int64_t c = p.ids[s * p.ids_stride + t];
+  if (c < 0 || c >= p.vocab) {
+    atomicOr(p.ticket + 1, unsigned(MLLM_GRPO_DEV_ID_CLAMPED));
+    if (p.device_status) atomicOr(p.device_status, MLLM_GRPO_DEV_ID_CLAMPED);
+  }
   const float2* st = p.stats + n * p.splits;
   float M = st[0].x;
   for (int k = 1; k < p.splits; ++k) M = fmaxf(M, st[k].x);
@@ -213,17 +223,18 @@ struct SeqSums {
   double diff, lp, count;
 };
 
+// This thread's share (tid of nt) of sequence s.
 template <bool LOGPS>
 __device__ __forceinline__ SeqSums sequence_sums(const Params& p, int64_t s, int tid, int nt) {
   SeqSums a{0.0, 0.0, 0.0};
   const bool per_token = p.ref != nullptr && !p.ref_per_sequence;
+#pragma unroll 2
   for (int64_t t = tid; t < p.scored_rows; t += nt) {
-    const int64_t n = s * p.scored_rows + t;
     float m;
-    if (!live_token(p, n, &m)) continue;
-    const double lp = token_logp<LOGPS>(p, n);
+    if (!live_token(p, s, t, &m)) continue;
+    const double lp = token_logp<LOGPS>(p, s, t);
     a.lp += double(m) * lp;
-    a.diff += double(m) * (per_token ? lp - double(p.ref[n]) : lp);
+    a.diff += double(m) * (per_token ? lp - double(p.ref[s * p.scored_rows + t]) : lp);
     a.count += double(m);
   }
   return a;
@@ -234,6 +245,7 @@ __device__ __forceinline__ double warp_add(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ SeqSums warp_add(SeqSums a) { return SeqSums{warp_add(a.diff), warp_add(a.lp), warp_add(a.count)}; }
 
 // log(1 + e^z) without overflow
 __device__ __forceinline__ double softplus(double z) { return z > 0.0 ? z + log1p(exp(-z)) : log1p(exp(z)); }
@@ -289,9 +301,8 @@ __device__ __forceinline__ float2 finish_pair(const Params& p, int64_t pair, Seq
 __device__ __forceinline__ void write_dlogps(const Params& p, int64_t s, float coef, int tid, int nt) {
   const float gs = p.grad_scale_dev ? *p.grad_scale_dev : p.grad_scale;
   for (int64_t t = tid; t < p.scored_rows; t += nt) {
-    const int64_t n = s * p.scored_rows + t;
     float m;
-    p.dlogps[n] = live_token(p, n, &m) ? coef * m * gs : 0.f;
+    p.dlogps[s * p.scored_rows + t] = live_token(p, s, t, &m) ? coef * m * gs : 0.f;
   }
 }
 
@@ -313,60 +324,79 @@ __device__ __forceinline__ void reduce_loss(const Params& p, double* red) {
   if (threadIdx.x == 0) *p.loss = float(a / double(p.total_dev ? *p.total_dev : p.total));
 }
 
-// One CTA per pair.  From logits the CTA that finishes last adds the pairs up (the ticket was zeroed by the stats
-// launch before this one); from log-probs the sum has a launch of its own, since nothing ran before to zero it.
+// One CTA per pair, half of it per answer.  From logits the CTA that finishes last adds the pairs up (the ticket was
+// zeroed by the stats launch before this one); from log-probs the sum has a launch of its own, since nothing ran before
+// to zero it.
 template <bool LOGPS>
 __global__ void __launch_bounds__(kPairThreads) pref_pairs_kernel(const Params p) {
+  constexpr int kHalf = kPairThreads / 2, kHalfWarps = kHalf / 32;
   __shared__ double red[32];
+  __shared__ SeqSums sums[2 * kHalfWarps];
   __shared__ float2 k_shared;
   __shared__ bool last;
-  const int64_t pair = blockIdx.x;
-  SeqSums c = sequence_sums<LOGPS>(p, pair, threadIdx.x, kPairThreads);
-  SeqSums r = sequence_sums<LOGPS>(p, p.n_pairs + pair, threadIdx.x, kPairThreads);
-  c.diff = block_sum(c.diff, red);
-  c.lp = block_sum(c.lp, red);
-  c.count = block_sum(c.count, red);
-  r.diff = block_sum(r.diff, red);
-  r.lp = block_sum(r.lp, red);
-  r.count = block_sum(r.count, red);
-  if (threadIdx.x == 0) k_shared = finish_pair(p, pair, c, r);
-  if (LOGPS) {
-    if (p.dlogps == nullptr) return;
-    __syncthreads();
-    write_dlogps(p, pair, k_shared.x, threadIdx.x, kPairThreads);
-    write_dlogps(p, p.n_pairs + pair, k_shared.y, threadIdx.x, kPairThreads);
-    return;
-  }
+  const int side = threadIdx.x / kHalf, tid = threadIdx.x % kHalf;
+  const int64_t pair = blockIdx.x, s = side * p.n_pairs + pair;
+  const SeqSums mine = warp_add(sequence_sums<LOGPS>(p, s, tid, kHalf));
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = mine;
+  __syncthreads();
   if (threadIdx.x == 0) {
-    __threadfence();
-    last = atomicAdd(p.ticket, 1u) == unsigned(p.n_pairs - 1);
-    __threadfence();
+    SeqSums a[2];
+    for (int k = 0; k < 2; ++k) {
+      a[k] = sums[k * kHalfWarps];
+      for (int w = 1; w < kHalfWarps; ++w) {
+        a[k].diff += sums[k * kHalfWarps + w].diff;
+        a[k].lp += sums[k * kHalfWarps + w].lp;
+        a[k].count += sums[k * kHalfWarps + w].count;
+      }
+    }
+    k_shared = finish_pair(p, pair, a[0], a[1]);
+    if (!LOGPS) {
+      __threadfence();
+      last = atomicAdd(p.ticket, 1u) == unsigned(p.n_pairs - 1);
+      __threadfence();
+    }
   }
   __syncthreads();
-  if (last) reduce_loss(p, red);
+  if (LOGPS) {
+    if (p.dlogps) write_dlogps(p, s, side ? k_shared.y : k_shared.x, tid, kHalf);
+  } else if (last) {
+    reduce_loss(p, red);
+    if (threadIdx.x == 0 && p.call_status) *p.call_status = int32_t(atomicOr(p.ticket + 1, 0u));
+  }
 }
 
-// Few tokens: one CTA, one warp per pair, loss included.
-__global__ void __launch_bounds__(1024) pref_logps_one_cta_kernel(const Params p) {
+// Few tokens: one CTA, loss included.  A sequence has 32 / sequences warps (one at least).
+__global__ void __launch_bounds__(1024) pref_logps_one_cta_kernel(const Params p, const int warps_per_seq) {
   __shared__ double red[32];
+  __shared__ SeqSums sums[32];
+  __shared__ float coef[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int64_t pair = warp; pair < p.n_pairs; pair += 32) {
-    SeqSums c = sequence_sums<true>(p, pair, lane, 32);
-    SeqSums r = sequence_sums<true>(p, p.n_pairs + pair, lane, 32);
-    c.diff = warp_add(c.diff);
-    c.lp = warp_add(c.lp);
-    c.count = warp_add(c.count);
-    r.diff = warp_add(r.diff);
-    r.lp = warp_add(r.lp);
-    r.count = warp_add(r.count);
-    float2 k = make_float2(0.f, 0.f);
-    if (lane == 0) k = finish_pair(p, pair, c, r);
-    k.x = __shfl_sync(0xffffffffu, k.x, 0);
-    k.y = __shfl_sync(0xffffffffu, k.y, 0);
-    if (p.dlogps) {
-      write_dlogps(p, pair, k.x, lane, 32);
-      write_dlogps(p, p.n_pairs + pair, k.y, lane, 32);
+  const int at_once = 32 / warps_per_seq;  // sequences, an even number: chosen answers first, then the same pairs' rejected
+  const int half = at_once / 2, slot = warp / warps_per_seq, sub = warp % warps_per_seq;
+  for (int64_t pair0 = 0; pair0 < p.n_pairs; pair0 += half) {
+    const int64_t pair = pair0 + slot % half, s = pair + (slot / half) * p.n_pairs;
+    const bool in = pair < p.n_pairs;
+    SeqSums mine{0.0, 0.0, 0.0};
+    if (in) mine = warp_add(sequence_sums<true>(p, s, sub * 32 + lane, warps_per_seq * 32));
+    if (lane == 0) sums[warp] = mine;
+    __syncthreads();
+    if (threadIdx.x < half && pair0 + threadIdx.x < p.n_pairs) {
+      SeqSums a[2];
+      for (int k = 0; k < 2; ++k) {
+        const SeqSums* q = sums + (k * half + threadIdx.x) * warps_per_seq;
+        a[k] = q[0];
+        for (int w = 1; w < warps_per_seq; ++w) {
+          a[k].diff += q[w].diff;
+          a[k].lp += q[w].lp;
+          a[k].count += q[w].count;
+        }
+      }
+      const float2 k = finish_pair(p, pair0 + threadIdx.x, a[0], a[1]);
+      coef[threadIdx.x] = k.x;
+      coef[half + threadIdx.x] = k.y;
     }
+    __syncthreads();
+    if (in && p.dlogps) write_dlogps(p, s, coef[slot], sub * 32 + lane, warps_per_seq * 32);
   }
   __syncthreads();
   reduce_loss(p, red);
@@ -392,13 +422,12 @@ __global__ void __launch_bounds__(THREADS) pref_dlogits_kernel(const Params p) {
   float g = 0.f, lse = 0.f;
   int64_t cl = -1;
   if (t < p.scored_rows) {
-    const int64_t n = b * p.scored_rows + t;
     float m;
-    if (live_token(p, n, &m)) {
+    if (live_token(p, b, t, &m)) {
       const float gs = p.grad_scale_dev ? *p.grad_scale_dev : p.grad_scale;
       g = -p.coef[b] * m * gs;
-      lse = p.lse[n];
-      int64_t c = p.ids[n];
+      lse = p.lse[b * p.scored_rows + t];
+      int64_t c = p.ids[b * p.ids_stride + t];
       c = c < 0 ? 0 : (c >= p.vocab ? p.vocab - 1 : c);
       cl = c - c0;
     }
@@ -489,6 +518,8 @@ static int bind(const mllm_grpo_preference_args* a, unsigned need, Params* p) {
     p->splits = int((a->vocab + p->split_cols - 1) / p->split_cols);  // none of them empty
     if (2 * a->n_pairs * a->seq_rows > kMost / p->splits) return MLLM_GRPO_ERR_TOO_LARGE;
   }
+  if ((a->ids_stride != 0 && a->ids_stride < a->scored_rows) || (a->mask_stride != 0 && a->mask_stride < a->scored_rows))
+    return MLLM_GRPO_ERR_BAD_SHAPE;
   if (a->kind < 0 || a->kind > MLLM_GRPO_PREFERENCE_IPO || !(a->beta > 0.f) || !(a->softcap >= 0.f) ||
       !(a->label_smoothing >= 0.f && a->label_smoothing <= 0.5f) ||
       (a->label_smoothing != 0.f && a->kind != MLLM_GRPO_PREFERENCE_SIGMOID))
@@ -500,7 +531,8 @@ static int bind(const mllm_grpo_preference_args* a, unsigned need, Params* p) {
   if ((need & kLogps) && !a->token_logps) return MLLM_GRPO_ERR_NULL_POINTER;
   if ((need & kBackward) && !a->dlogits) return MLLM_GRPO_ERR_NULL_POINTER;
   const void* words[] = {a->chosen_ids, a->token_logps, a->mask, a->ref_logps, a->pair_weights, a->total_pairs_dev,
-                         a->grad_scale_dev, a->loss, a->rewards, a->sequence_logps, a->dtoken_logps, a->device_status};
+                         a->grad_scale_dev, a->loss, a->rewards, a->sequence_logps, a->dtoken_logps, a->device_status,
+                         a->call_status};
   for (const void* q : words)
     if (!aligned(q, 4)) return MLLM_GRPO_ERR_ALIGNMENT;
   if (!aligned(a->logits, 2) || !aligned(a->dlogits, 2) || !aligned(a->workspace, 16)) return MLLM_GRPO_ERR_ALIGNMENT;
@@ -522,6 +554,9 @@ static int bind(const mllm_grpo_preference_args* a, unsigned need, Params* p) {
   p->ids = a->chosen_ids;
   p->logps = a->token_logps;
   p->mask = a->mask;
+  p->mask_int = a->mask_int;
+  p->ids_stride = a->ids_stride ? a->ids_stride : a->scored_rows;
+  p->mask_stride = a->mask_stride ? a->mask_stride : a->scored_rows;
   p->ref = a->ref_logps;
   p->weights = a->pair_weights;
   p->total_dev = a->total_pairs_dev;
@@ -532,6 +567,7 @@ static int bind(const mllm_grpo_preference_args* a, unsigned need, Params* p) {
   p->dlogps = a->dtoken_logps;
   p->dlogits = static_cast<uint16_t*>(a->dlogits);
   p->device_status = a->device_status;
+  p->call_status = a->call_status;
   char* w = static_cast<char*>(a->workspace);
   p->ticket = reinterpret_cast<unsigned int*>(w);
   w += 16;
@@ -593,7 +629,9 @@ int mllm_grpo_preference_logps(const mllm_grpo_preference_args* args, void* stre
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (2 * p.n_pairs * p.scored_rows <= pref::kOneCtaTokens) {
-    pref::pref_logps_one_cta_kernel<<<1, 1024, 0, s>>>(p);
+    int per = 1;  // warps per sequence: 16 for one pair
+    while (per < 16 && per * 2 * 2 * p.n_pairs <= 32) per *= 2;
+    pref::pref_logps_one_cta_kernel<<<1, 1024, 0, s>>>(p, per);
     e = pref::done();
   } else {
     pref::pref_pairs_kernel<true><<<unsigned(p.n_pairs), pref::kPairThreads, 0, s>>>(p);

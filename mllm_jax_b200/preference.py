@@ -41,69 +41,91 @@ class PreferenceConfig:
 def _f32(t: Optional[torch.Tensor], dev, shapes, name: str) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if tuple(t.shape) not in shapes:
-        raise ValueError(f"{name} must have shape {' or '.join(str(s) for s in shapes)}, got {tuple(t.shape)}")
+    if t.shape not in shapes:
+        raise ValueError(f"{name} must have shape {' or '.join(str(tuple(s)) for s in shapes)}, got {tuple(t.shape)}")
+    if t.dtype is torch.float32 and t.device == dev and t.is_contiguous():
+        return t
     return t.to(device=dev, dtype=torch.float32).contiguous()
+
+
+def _rows(t: torch.Tensor, dev, dtypes) -> torch.Tensor:
+    """A [B, T] tensor of one of `dtypes` whose rows are contiguous and any distance apart (a view where possible)."""
+    if t.dtype not in dtypes or t.device != dev:
+        t = t.to(device=dev, dtype=dtypes[0])
+    B, T = t.shape
+    if (T > 1 and t.stride(1) != 1) or (B > 1 and t.stride(0) < T):
+        t = t.contiguous()
+    return t
 
 
 class PreferenceProblem:
     """Device buffers of one call, laid out as the C ABI wants them; keeps references so that they outlive the launch."""
 
     def __init__(self, sequences: int, T: int, dev, mask, ref, pair_weights, total_pairs, cfg: PreferenceConfig):
-        if sequences < 2 or sequences % 2:
-            raise ValueError(f"the batch holds chosen and rejected answers of pairs: {sequences} sequences is not a "
+        B, P = sequences, sequences // 2
+        if B < 2 or B % 2:
+            raise ValueError(f"the batch holds chosen and rejected answers of pairs: {B} sequences is not a "
                              "positive even number")
         if T < 1:
             raise ValueError("there is no scored position")
-        if cfg.loss_type not in _KINDS:
+        kind = _KINDS.get(cfg.loss_type)
+        if kind is None:
             raise ValueError(f"loss_type must be one of {sorted(_KINDS)}, got {cfg.loss_type!r}")
         if not cfg.beta > 0:
             raise ValueError(f"beta must be positive, got {cfg.beta}")
-        if not 0 <= cfg.label_smoothing <= 0.5 or (cfg.label_smoothing and cfg.loss_type != "sigmoid"):
+        if not 0 <= cfg.label_smoothing <= 0.5 or (cfg.label_smoothing and kind != 0):
             raise ValueError("label_smoothing must lie in [0, 0.5] and belongs to the sigmoid loss")
-        self.P, self.T, self.dev, self.cfg = sequences // 2, T, dev, cfg
-        B = sequences
-        self.mask = _f32(mask, dev, [(B, T)], "mask")
-        self.ref = _f32(ref, dev, [(B, T), (B,)], "ref_per_token_logps")
-        self.weights = _f32(pair_weights, dev, [(self.P,)], "pair_weights")
+        self.P, self.T, self.dev, self.cfg = P, T, dev, cfg
+        self.mask = None
+        if mask is not None:
+            if mask.shape != (B, T):
+                raise ValueError(f"mask must have shape {(B, T)}, got {tuple(mask.shape)}")
+            self.mask = _rows(mask, dev, (torch.float32, torch.int32))
+        self.ref = _f32(ref, dev, ((B, T), (B,)), "ref_per_token_logps")
+        self.weights = _f32(pair_weights, dev, ((P,),), "pair_weights")
         self.total_dev = None
-        self.total = float(self.P)
+        self.total = float(P)
         if isinstance(total_pairs, torch.Tensor):
             self.total_dev = total_pairs.to(device=dev, dtype=torch.float32).reshape(1)
         elif total_pairs is not None:
             self.total = float(total_pairs)
-        lib = _lib.load()
-        nbytes = int(lib.mllm_grpo_preference_workspace_bytes(self.P, T))
+        nbytes = _lib.load().mllm_grpo_preference_workspace_bytes(P, T)
         if nbytes == 0:
             raise ValueError(f"{B} x {T} scored positions are too many for one call")
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        out = torch.empty(1 + 4 * self.P, dtype=torch.float32, device=dev)
-        self.loss, self.rewards, self.sequence_logps = out[0], out[1:1 + B], out[1 + B:]
-        self.device_status = None
-        self.grad_scale = 1.0
-        a = self.a = _lib.PreferenceArgs()
-        a.n_pairs, a.seq_rows, a.scored_rows = self.P, T, T
-        a.kind, a.average = _KINDS[cfg.loss_type], int(cfg.average)
-        a.beta, a.label_smoothing = cfg.beta, cfg.label_smoothing
-        a.softcap = float(cfg.softcap) if cfg.softcap else 0.0
-        a.grad_scale, a.total_pairs = 1.0, self.total
-        a.mask = None if self.mask is None else self.mask.data_ptr()
-        a.ref_logps = None if self.ref is None else self.ref.data_ptr()
-        a.ref_per_sequence = int(self.ref is not None and self.ref.dim() == 1)
-        a.pair_weights = None if self.weights is None else self.weights.data_ptr()
-        a.total_pairs_dev = None if self.total_dev is None else self.total_dev.data_ptr()
-        a.loss, a.rewards = out.data_ptr(), self.rewards.data_ptr()
-        a.sequence_logps, a.workspace = self.sequence_logps.data_ptr(), self.workspace.data_ptr()
+        self.out = torch.empty(2 + 4 * P, dtype=torch.float32, device=dev)  # rewards, log-probs, loss, status
+        o = self.out.data_ptr()
+        self.a = _lib.PreferenceArgs(
+            n_pairs=P, seq_rows=T, scored_rows=T, kind=kind, average=bool(cfg.average), beta=cfg.beta,
+            label_smoothing=cfg.label_smoothing, softcap=float(cfg.softcap) if cfg.softcap else 0.0, grad_scale=1.0,
+            total_pairs=self.total, rewards=o, sequence_logps=o + 4 * B, loss=o + 8 * B, call_status=o + 8 * B + 4,
+            workspace=self.workspace.data_ptr())
+        a = self.a
+        if self.mask is not None:
+            a.mask, a.mask_int = self.mask.data_ptr(), self.mask.dtype is torch.int32
+            a.mask_stride = self.mask.stride(0) if B > 1 else 0
+        if self.ref is not None:
+            a.ref_logps, a.ref_per_sequence = self.ref.data_ptr(), self.ref.dim() == 1
+        if self.weights is not None:
+            a.pair_weights = self.weights.data_ptr()
+        if self.total_dev is not None:
+            a.total_pairs_dev = self.total_dev.data_ptr()
+
+    @property
+    def device_status(self) -> torch.Tensor:
+        """MLLM_GRPO_DEV_* bits of the forward from logits (an int32 on the device)."""
+        return self.out[-1:].view(torch.int32)
 
     def bind_logits(self, logits: torch.Tensor, ids: torch.Tensor, L: int) -> None:
         self.logits = logits
-        if tuple(ids.shape) != (2 * self.P, self.T):
+        if ids.shape != (2 * self.P, self.T):
             raise ValueError(f"token ids must have {2 * self.P}x{self.T} elements, got shape {tuple(ids.shape)}")
-        self.ids = ids.to(device=self.dev, dtype=torch.int32).contiguous()
-        self.device_status = torch.zeros(1, dtype=torch.int32, device=self.dev)
+        if ids.dtype is torch.int64:
+            ids = ids.clamp(-1, 2 ** 31 - 1)  # an id beyond 32 bits must not wrap to a valid one
+        self.ids = _rows(ids, self.dev, (torch.int32,))
         a = self.a
         a.seq_rows, a.vocab, a.row_stride = L, logits.shape[2], logits.stride(1)
-        a.logits, a.chosen_ids, a.device_status = logits.data_ptr(), self.ids.data_ptr(), self.device_status.data_ptr()
+        a.logits, a.chosen_ids, a.ids_stride = logits.data_ptr(), self.ids.data_ptr(), self.ids.stride(0)
 
     def bind_dlogits(self, dlogits: torch.Tensor) -> torch.Tensor:
         x = self.logits
@@ -118,9 +140,9 @@ class PreferenceProblem:
         _lib.launch(entry, self.a, self.dev)
 
     def outputs(self) -> dict:
-        P = self.P
-        return {"loss": self.loss, "chosen_rewards": self.rewards[:P], "rejected_rewards": self.rewards[P:],
-                "chosen_logps": self.sequence_logps[:P], "rejected_logps": self.sequence_logps[P:]}
+        good, bad, good_lp, bad_lp, rest = self.out.split((self.P, self.P, self.P, self.P, 2))
+        return {"loss": rest[0], "chosen_rewards": good, "rejected_rewards": bad, "chosen_logps": good_lp,
+                "rejected_logps": bad_lp}
 
 
 def _from_logits(logits, token_ids, mask, ref, shifted, cfg, pair_weights, total_pairs) -> PreferenceProblem:
@@ -175,12 +197,11 @@ class _PreferenceLoss(torch.autograd.Function):
         prob.run("mllm_grpo_preference_fwd")
         ctx.prob, ctx.inplace, ctx.spent = prob, inplace_backward, False
         ctx.save_for_backward(logits)  # a change of the logits between the sweeps is an error
-        ctx.mark_non_differentiable(prob.rewards, prob.sequence_logps)
-        return prob.loss.clone(), prob.rewards, prob.sequence_logps
+        return prob.out[-2].clone()
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, grad_loss, _g_rewards, _g_logps):
+    def backward(ctx, grad_loss):
         prob: PreferenceProblem = ctx.prob
         (logits,) = ctx.saved_tensors
         if ctx.spent:
@@ -202,10 +223,8 @@ def preference_loss(logits: torch.Tensor, input_ids: torch.Tensor, labels: Optio
     input_ids / labels [2P, L], reference log-probs [2P, L-1], [2P] or None (see `preference_value_and_grad`).
     Only `loss` is differentiable; rewards and log-probs are detached."""
     prob = _from_logits(logits.detach(), input_ids, labels, ref_per_token_logps, True, cfg, pair_weights, total_pairs)
-    P = prob.P
-    loss, rewards, lps = _PreferenceLoss.apply(logits, prob, inplace_backward)
-    return {"loss": loss, "chosen_rewards": rewards[:P], "rejected_rewards": rewards[P:], "chosen_logps": lps[:P],
-            "rejected_logps": lps[P:]}
+    loss = _PreferenceLoss.apply(logits, prob, inplace_backward)
+    return {**prob.outputs(), "loss": loss, "problem": prob}
 
 
 def preference_logps_value_and_grad(per_token_logps: torch.Tensor, mask: Optional[torch.Tensor],
@@ -222,7 +241,7 @@ def preference_logps_value_and_grad(per_token_logps: torch.Tensor, mask: Optiona
         raise ValueError(f"per_token_logps must be [2P, T], got shape {tuple(x.shape)}")
     prob = PreferenceProblem(x.shape[0], x.shape[1], x.device, mask, ref_per_token_logps, pair_weights, total_pairs,
                              cfg or PreferenceConfig())
-    prob.logps = x.detach().to(torch.float32).contiguous()
+    prob.logps = _f32(x.detach(), x.device, (x.shape,), "per_token_logps")
     dlogps = torch.empty_like(prob.logps)
     prob.a.token_logps, prob.a.dtoken_logps = prob.logps.data_ptr(), dlogps.data_ptr()
     prob.a.grad_scale = float(grad_scale)
@@ -234,19 +253,16 @@ def preference_logps_value_and_grad(per_token_logps: torch.Tensor, mask: Optiona
 
 class _PreferenceLogpsLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logps, mask, ref, kwargs):
-        out = preference_logps_value_and_grad(logps, mask, ref, **kwargs)
-        prob = out["problem"]
+    def forward(ctx, logps, out):
         ctx.save_for_backward(out["dlogps"])
         ctx.dtype = logps.dtype
-        ctx.mark_non_differentiable(prob.rewards, prob.sequence_logps)
-        return prob.loss.clone(), prob.rewards, prob.sequence_logps
+        return out["loss"].clone()
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, grad_loss, _g_rewards, _g_logps):
+    def backward(ctx, grad_loss):
         (d,) = ctx.saved_tensors
-        return (grad_loss * d).to(ctx.dtype), None, None, None
+        return (grad_loss * d).to(ctx.dtype), None
 
 
 def preference_loss_from_logps(per_token_logps: torch.Tensor, mask: Optional[torch.Tensor],
@@ -255,8 +271,6 @@ def preference_loss_from_logps(per_token_logps: torch.Tensor, mask: Optional[tor
                                total_pairs=None) -> dict:
     """`preference_logps_value_and_grad` as a differentiable function of the log-probs (the gradient is formed with
     the loss; backward applies the cotangent)."""
-    P = per_token_logps.shape[0] // 2
-    loss, rewards, lps = _PreferenceLogpsLoss.apply(per_token_logps, mask, ref_per_token_logps,
-                                                    dict(cfg=cfg, pair_weights=pair_weights, total_pairs=total_pairs))
-    return {"loss": loss, "chosen_rewards": rewards[:P], "rejected_rewards": rewards[P:], "chosen_logps": lps[:P],
-            "rejected_logps": lps[P:]}
+    out = preference_logps_value_and_grad(per_token_logps, mask, ref_per_token_logps, cfg=cfg, pair_weights=pair_weights,
+                                          total_pairs=total_pairs)
+    return {**{k: v for k, v in out.items() if k != "dlogps"}, "loss": _PreferenceLogpsLoss.apply(per_token_logps, out)}
