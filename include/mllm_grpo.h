@@ -453,7 +453,7 @@ typedef struct mllm_lm_head_fp8_args {
   int64_t out_stride;     /* elements between rows of out, >= vocab (product) */
   int64_t vocab_start, vocab_total; /* partials: as in mllm_lm_head_args */
   float softcap;          /* partials */
-  int32_t reserved;       /* 0 */
+  float temperature;      /* partials, per_token_logps: > 0, or 0 for 1 */
   int32_t out_dtype;      /* product: MLLM_GRPO_BF16, _F16 or _F32 */
   const void* hidden;         /* e4m3 [M, K], 16-byte aligned */
   const float* hidden_scales; /* [M, ceil(K / 128)] */
@@ -462,12 +462,16 @@ typedef struct mllm_lm_head_fp8_args {
   void* out;                  /* product */
   const int32_t* chosen_ids;  /* partials: [M] */
   void* partials;             /* partials: mllm_lm_head_fp8_partials_bytes(n_rows, vocab) bytes, 16-byte aligned */
+  float* per_token_logps;     /* partials: [M] or NULL, for an unsharded head: (chosen logit - lse) / temperature */
+  float* token_entropy;       /* partials: [M] or NULL, at temperature 1: lse - (sum e*y) / sumexp */
+  float* lse;                 /* partials: [M] or NULL */
   int32_t* device_status;     /* optional */
 } mllm_lm_head_fp8_args;
 int mllm_lm_head_fp8_matmul(const mllm_lm_head_fp8_args* args, void* stream);
 /* mllm_lm_head_partials with both operands in 8 bits.  The first n_rows records of `partials` are the rows' merged
  * (max, sumexp, sum e*y, chosen-or-0), to go through mllm_grpo_combine with n_shards = 1 (or, all-gathered over a
- * sharded head's ranks, n_shards = ranks); the rest of the buffer is scratch. */
+ * sharded head's ranks, n_shards = ranks); the rest of the buffer is scratch.  A caller that only wants log-probs (the
+ * reference-model pass) has them from this call. */
 int mllm_lm_head_fp8_partials(const mllm_lm_head_fp8_args* args, void* stream);
 int64_t mllm_lm_head_fp8_partials_bytes(int64_t n_rows, int64_t vocab);
 

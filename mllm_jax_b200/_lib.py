@@ -132,9 +132,11 @@ class Fp8Args(C.Structure):
         ("struct_size", C.c_uint64),
         ("n_rows", C.c_int64), ("vocab", C.c_int64), ("hidden_dim", C.c_int64), ("hidden_stride", C.c_int64),
         ("weight_stride", C.c_int64), ("out_stride", C.c_int64), ("vocab_start", C.c_int64),
-        ("vocab_total", C.c_int64), ("softcap", C.c_float), ("reserved", C.c_int32), ("out_dtype", C.c_int32),
+        ("vocab_total", C.c_int64), ("softcap", C.c_float), ("temperature", C.c_float),
+        ("out_dtype", C.c_int32),
         ("hidden", C.c_void_p), ("hidden_scales", C.c_void_p), ("weight", C.c_void_p), ("weight_scales", C.c_void_p),
-        ("out", C.c_void_p), ("chosen_ids", C.c_void_p), ("partials", C.c_void_p), ("device_status", C.c_void_p),
+        ("out", C.c_void_p), ("chosen_ids", C.c_void_p), ("partials", C.c_void_p), ("per_token_logps", C.c_void_p),
+        ("token_entropy", C.c_void_p), ("lse", C.c_void_p), ("device_status", C.c_void_p),
     ]
 
 

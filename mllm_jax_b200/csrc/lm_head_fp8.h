@@ -19,6 +19,10 @@ struct Params {
   void* out;
   const int32_t* chosen_ids;
   float4* partials;  // [1 + ranges, n_rows]: the merged entry, then one entry per column range
+  float inv_temperature;
+  float* logps;
+  float* entropy;
+  float* lse;
   int32_t* device_status;
 };
 

@@ -519,20 +519,27 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       if (!STATS) {
         store_rows<O, CW, T::kStoreBytes>(p, &map_out, acc, int64_t(m_tile) * kBM + quarter * 32, n0, valid, my_store, lane);
       } else if (valid > 0) {
-        const int64_t c_local = c >= 0 ? c - n0 : -1;
         float y[CW];
-        float cm = kNegInit;
 #pragma unroll
-        for (int j = 0; j < CW / 2; ++j) {
-          unpack2(acc[j], y[2 * j], y[2 * j + 1]);
-        }
+        for (int j = 0; j < CW / 2; ++j) unpack2(acc[j], y[2 * j], y[2 * j + 1]);
+        if (cap) {
 #pragma unroll
-        for (int j = 0; j < CW; ++j) {
-          if (cap) y[j] = sc.y(y[j]);
-          if (j == c_local) yc = y[j];
-          y[j] = j < valid ? y[j] : kNegInit;
-          cm = fmaxf(cm, y[j]);
+          for (int j = 0; j < CW; ++j) y[j] = sc.y(y[j]);
         }
+        // a chosen column is in few tiles, the end of the vocabulary in one: whole warps skip looking for them
+        const int64_t c_local = c >= 0 ? c - n0 : -1;
+        if (__any_sync(0xffffffffu, c_local >= 0 && c_local < CW)) {
+#pragma unroll
+          for (int j = 0; j < CW; ++j)
+            if (j == c_local) yc = y[j];
+        }
+        if (valid < CW) {
+#pragma unroll
+          for (int j = 0; j < CW; ++j) y[j] = j < valid ? y[j] : kNegInit;
+        }
+        float cm = y[0];
+#pragma unroll
+        for (int j = 1; j < CW; ++j) cm = fmaxf(cm, y[j]);
         if (cm > m) {
           const float r = ex2f((m - cm) * kLog2e);
           s *= r;
@@ -579,8 +586,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   }
 }
 
-// Partials of all column ranges of a row -> one (entry 0 of the buffer): 32 rows per CTA, eight threads per row.
-__global__ void __launch_bounds__(256) merge_kernel(float4* partials, int64_t n_rows, int entries) {
+// Partials of all column ranges of a row -> one (entry 0 of the buffer) and what follows from it: 32 rows per CTA, eight
+// threads per row.
+__global__ void __launch_bounds__(256) merge_kernel(const Params p, int entries) {
+  float4* const partials = p.partials;
+  const int64_t n_rows = p.n_rows;
   __shared__ float4 part[8][32];
   const int r = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int64_t row = int64_t(blockIdx.x) * 32 + r;
@@ -605,6 +615,10 @@ __global__ void __launch_bounds__(256) merge_kernel(float4* partials, int64_t n_
   if (g == 0 && row < n_rows) {
     for (int i = 1; i < 8; ++i) add(part[i][r]);
     partials[row] = make_float4(m, s, u, yc);
+    const float lse = m + logf(s);
+    if (p.logps) p.logps[row] = (yc - lse) * p.inv_temperature;
+    if (p.entropy) p.entropy[row] = lse - u / s;
+    if (p.lse) p.lse[row] = lse;
   }
 }
 
@@ -796,8 +810,20 @@ int mllm_lm_head_fp8_partials(const mllm_lm_head_fp8_args* a, void* stream) {
   if (a->n_rows == 0) return MLLM_GRPO_ERR_BAD_SHAPE;
   if (!a->chosen_ids || !a->partials) return MLLM_GRPO_ERR_NULL_POINTER;
   if (a->vocab_start < 0 || (a->vocab_total > 0 && a->vocab_start + a->vocab > a->vocab_total)) return MLLM_GRPO_ERR_BAD_SHAPE;
-  if (!(a->softcap >= 0.f)) return MLLM_GRPO_ERR_BAD_ATTRIBUTE;
-  if (!fp8::aligned(a->partials, 16) || !fp8::aligned(a->chosen_ids, 4)) return MLLM_GRPO_ERR_ALIGNMENT;
+  if (!(a->softcap >= 0.f) || !(a->temperature >= 0.f)) return MLLM_GRPO_ERR_BAD_ATTRIBUTE;
+  if (!fp8::aligned(a->partials, 16) || !fp8::aligned(a->chosen_ids, 4) || !fp8::aligned(a->per_token_logps, 4) ||
+      !fp8::aligned(a->token_entropy, 4) || !fp8::aligned(a->lse, 4))
+    return MLLM_GRPO_ERR_ALIGNMENT;
+  const float temperature = a->temperature > 0.f ? a->temperature : 1.0f;
+  if (a->token_entropy && temperature != 1.0f) return MLLM_GRPO_ERR_UNSUPPORTED;
+  // a shard of the vocabulary does not know a row's log-sum-exp
+  if ((a->per_token_logps || a->token_entropy || a->lse) &&
+      (a->vocab_start != 0 || (a->vocab_total > 0 && a->vocab_total != a->vocab)))
+    return MLLM_GRPO_ERR_UNSUPPORTED;
+  p.inv_temperature = 1.0f / temperature;
+  p.logps = a->per_token_logps;
+  p.entropy = a->token_entropy;
+  p.lse = a->lse;
   p.vocab_start = a->vocab_start;
   p.vocab_total = a->vocab_total > 0 ? a->vocab_total : a->vocab_start + a->vocab;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -806,7 +832,7 @@ int mllm_lm_head_fp8_partials(const mllm_lm_head_fp8_args* a, void* stream) {
   if (st) return st;
   int per, splits;
   fp8::fold_plan(a->n_rows, a->vocab, &per, &splits);
-  fp8::merge_kernel<<<unsigned((a->n_rows + 31) / 32), 256, 0, s>>>(p.partials, a->n_rows, splits * 2);
+  fp8::merge_kernel<<<unsigned((a->n_rows + 31) / 32), 256, 0, s>>>(p, splits * 2);
   count_launch();
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);

@@ -82,8 +82,7 @@ def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]
     N = B * T
     lib = _lib.load()
     if fp8:
-        with torch.cuda.device(dev):
-            hq = quantize_fp8(hidden.reshape(N, H), block=(1, 128))
+        hq = quantize_fp8(hidden.reshape(N, H), block=(1, 128))
         a = _bind(hq, weight)
         splits, nbytes = 1, int(lib.mllm_lm_head_fp8_partials_bytes(N, V))
     else:
@@ -95,6 +94,9 @@ def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]
     elif workspace.numel() * workspace.element_size() < nbytes or workspace.data_ptr() % 16:
         raise ValueError(f"workspace must hold {nbytes} bytes at a 16-byte aligned address")
     forward_only = advantages is None
+    if fp8 and forward_only and group is None and vocab_start == 0 and vocab_total in (None, V) and \
+            total_valid_token_count is None and old_per_token_logps is None and ref_per_token_logps is None:
+        return _fp8_logprobs(a, hq, weight, token_ids, cfg, workspace, B, T, dev)
     if forward_only:
         advantages = torch.zeros(B, dtype=torch.float32, device=dev)
     # side arrays, outputs and residuals exactly as for materialised logits; no logits tensor is bound
@@ -133,6 +135,32 @@ def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]
     if not forward_only:
         out["loss"] = prob.loss.reshape(())
     return out
+
+
+class _LogprobsCall:
+    """What a log-probs-only call keeps alive, and its status word."""
+
+    def __init__(self, device_status, *keep):
+        self.device_status, self._keepalive = device_status, keep
+
+
+def _fp8_logprobs(a, hq: Fp8Blocks, weight: Fp8Blocks, token_ids, cfg: LossConfig, workspace, B: int, T: int, dev) -> dict:
+    """Log-probs, entropies and log-sum-exps of an unsharded 8-bit head: three launches, the last of which merges the
+    vocabulary ranges and writes the results."""
+    if token_ids.numel() != B * T:
+        raise ValueError(f"chosen ids must have {B}x{T} elements, got shape {tuple(token_ids.shape)}")
+    ids = token_ids.to(device=dev, dtype=torch.int32).contiguous()
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = torch.empty(3, B, T, dtype=torch.float32, device=dev)
+    lp, ent, lse = out.unbind(0)
+    a.chosen_ids, a.partials, a.device_status = ids.data_ptr(), workspace.data_ptr(), status.data_ptr()
+    a.softcap, a.temperature = float(cfg.softcap) if cfg.softcap else 0.0, cfg.temperature
+    a.per_token_logps, a.lse = lp.data_ptr(), lse.data_ptr()
+    if cfg.compute_entropy:
+        a.token_entropy = ent.data_ptr()
+    _lib.launch("mllm_lm_head_fp8_partials", a, dev)
+    return {"per_token_logps": lp, "token_entropy": ent if cfg.compute_entropy else None, "lse": lse,
+            "problem": _LogprobsCall(status, hq, weight, ids, workspace), "splits": 1}
 
 
 def linear_grpo_value_and_grad(hidden: torch.Tensor, weight: torch.Tensor, token_ids: torch.Tensor,

@@ -175,6 +175,12 @@ def test_folded_head(cuda, B, T, H, V, cap):
     e_sum = 3 * 2.0 ** -20 + 2.0 ** -22 + (min(V, 16384) / 64 + 600) * 2.0 ** -24 + 4 * 2.0 ** -19
     R.assert_within(out["lse"].view(-1), lse, worst + e_sum, "lse")
     R.assert_within(out["per_token_logps"].view(-1), lp, 2 * worst + e_sum, "log-probs")
+    # the two-step form (combine after the partials, as a loss or a sharded head takes it) agrees
+    full = lm_head_forward(hidden, w, ids, None, torch.ones(B, device=cuda), cfg=G.LossConfig(softcap=cap))
+    R.assert_within(full["per_token_logps"].view(-1), out["per_token_logps"].view(-1).double(), 4 * 2.0 ** -19, "combined")
+    R.assert_within(full["token_entropy"].view(-1), out["token_entropy"].view(-1).double(), 4 * 2.0 ** -19, "combined entropy")
+    cold = lm_head_forward(hidden, w, ids, cfg=G.LossConfig(softcap=cap, temperature=0.5, compute_entropy=False))
+    assert cold["token_entropy"] is None and torch.equal(cold["per_token_logps"], 2 * out["per_token_logps"])
     # entropy = lse - U / S: U has the terms' relative error times |y|
     R.assert_within(out["token_entropy"].view(-1), ent, 2 * worst * (1 + y.abs().amax(1)) + e_sum * (2 + (p * y.abs()).sum(1)), "entropy")
 

@@ -167,6 +167,10 @@ def test_fp8_entry_points_ask_for_what_they_read(built_lib):
     assert _status("mllm_lm_head_fp8_partials", _fp8(partials=0x1008)) == 5
     assert _status("mllm_lm_head_fp8_partials", _fp8(vocab_start=1, vocab_total=100)) == 2
     assert _status("mllm_lm_head_fp8_partials", _fp8(softcap=-1.0)) == 3
+    assert _status("mllm_lm_head_fp8_partials", _fp8(temperature=-1.0)) == 3
+    assert _status("mllm_lm_head_fp8_partials", _fp8(temperature=0.7, token_entropy=0x1000)) == 7
+    assert _status("mllm_lm_head_fp8_partials", _fp8(vocab_total=200, lse=0x1000)) == 7
+    assert _status("mllm_lm_head_fp8_partials", _fp8(per_token_logps=0x1002)) == 5
     assert lib.mllm_lm_head_fp8_partials_bytes(0, 5) == 0 and lib.mllm_lm_head_fp8_partials_bytes(300, 151936) >= 300 * 16 * 2
 
 
