@@ -17,6 +17,7 @@
 #include <cuda_fp16.h>
 
 #include <cstring>
+#include <mutex>
 
 #include "grpo_cluster.cuh"
 #include "grpo_common.cuh"
@@ -108,13 +109,12 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const LookupParams p) 
 }
 
 // ---------------------------------------------------------------------------------------------
-// Stable radix sort of (id, token) by one cluster of eight CTAs (one CTA for up to 4096 pairs), 9 bits a pass.  CTA r
-// owns the r-th eighth of the pairs, in tiles of 4096, 128 consecutive pairs per warp.  Inside a tile a pair's place among
+// Stable radix sort of (id, token) by one cluster of eight CTAs (one CTA for up to 4096 pairs, 16 beyond 32768), 9 bits a
+// pass.  CTA r owns the r-th eighth of the pairs, in tiles of 4096, 128 consecutive pairs per warp.  Inside a tile a pair's place among
 // its digit is found by the warp's match of equal digits (stable: lower lanes first) and the running counts of the warps
 // before it; all eight CTAs' digit counts through distributed shared memory give every digit its first place.  Two
 // passes: 12 us for up to 4096 pairs, 25 us for 32768.
 // ---------------------------------------------------------------------------------------------
-constexpr int kSortCtas = 8;      // of a cluster, for more than one tile
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kRounds = 4;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(128) run_kernel(const GradParams p, const uint
   }
   const uint32_t k = __shfl_sync(0xffffffffu, mine, 0);
   if (__shfl_sync(0xffffffffu, mine, 31) != k || k >= p.vocab) return;
-  const uint32_t c = blockIdx.y * 128 + threadIdx.x;
+  const uint32_t c = blockIdx.y * blockDim.x + threadIdx.x;
   const bool ok = c < row_vecs;
   float acc[EV] = {};
 #pragma unroll
@@ -625,12 +625,15 @@ static cudaError_t launch_lookup_t(const mllm_grpo_embedding_args* a, LookupPara
 template <typename T, int EV>
 static cudaError_t launch_runs(const GradParams& p, cudaStream_t s) {
   const uint32_t runs = (p.n + kRun - 1) / kRun;
-  const auto parts = [](uint32_t row_vecs) { return (row_vecs + 127) / 128 + 1; };
+  const auto go = [&](auto* kernel, uint32_t row_vecs) {
+    const uint32_t threads = row_vecs <= 32 ? 32 : (row_vecs <= 64 ? 64 : 128);
+    kernel<<<dim3(runs, (row_vecs + threads - 1) / threads + 1), threads, 0, s>>>(p, row_vecs);
+  };
   constexpr int kWide = 16 / int(sizeof(T));
   if (vec_of(p.hidden, kWide, p.grad, p.grad_stride, sizeof(T), p.run, p.hidden, 2) == kWide)
-    run_kernel<T, kWide><<<dim3(runs, parts(p.hidden / kWide)), 128, 0, s>>>(p, p.hidden / kWide);
+    go(run_kernel<T, kWide>, p.hidden / kWide);
   else
-    run_kernel<T, EV><<<dim3(runs, parts(p.row_vecs)), 128, 0, s>>>(p, p.row_vecs);
+    go(run_kernel<T, EV>, p.row_vecs);
   return done();
 }
 
@@ -710,11 +713,10 @@ static cudaError_t launch_grad_t(const mllm_grpo_embedding_args* a, GradParams p
 }
 
 static cudaError_t launch_sort(const SortParams& q, bool zero_rows, cudaStream_t s) {
-  const bool small = q.n <= uint32_t(kTile);
+  const int ctas = q.n <= uint32_t(kTile) ? 1 : (q.n <= uint32_t(8 * kTile) ? 8 : 16);
   // 16 rows' marks a thread, in whole clusters
   int64_t more = zero_rows ? (q.vocab + kSortThreads * 16 - 1) / (kSortThreads * 16) : 0;
   more = more > 128 ? 128 : more;
-  const int ctas = small ? 1 : kSortCtas;
   more = (more + ctas - 1) / ctas * ctas;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(ctas + more));
@@ -726,8 +728,19 @@ static cudaError_t launch_sort(const SortParams& q, bool zero_rows, cudaStream_t
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = small ? 0 : 1;
-  const cudaError_t e = small ? cudaLaunchKernelEx(&cfg, sort_kernel<1>, q) : cudaLaunchKernelEx(&cfg, sort_kernel<kSortCtas>, q);
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  if (ctas == 16) {
+    static std::once_flag once[64];
+    static cudaError_t err[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    std::call_once(once[dev], [&] {
+      err[dev] = cudaFuncSetAttribute(sort_kernel<16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    });
+    if (err[dev] != cudaSuccess) return err[dev];
+  }
+  const cudaError_t e = ctas == 1 ? cudaLaunchKernelEx(&cfg, sort_kernel<1>, q)
+                                  : (ctas == 8 ? cudaLaunchKernelEx(&cfg, sort_kernel<8>, q) : cudaLaunchKernelEx(&cfg, sort_kernel<16>, q));
   count_launch();
   return e;
 }

@@ -21,7 +21,7 @@ namespace grpo {
 namespace pref {
 
 constexpr int kMaxSplits = 32;
-constexpr int64_t kTargetCtas = 592;    // 4 per SM
+constexpr int64_t kTargetCtas = 4736;   // 32 per SM, about half of which have a masked row and leave
 constexpr int64_t kMinSplitCols = 8192; // 16 KB of a row per CTA at least
 constexpr int kPairThreads = 512;
 constexpr int64_t kOneCtaTokens = 16384;
