@@ -407,13 +407,13 @@ __global__ void __launch_bounds__(kPairThreads) pref_loss_kernel(const Params p)
   reduce_loss(p, red);
 }
 
-// Gradient of one row (or its split); rows without a coefficient are written as zeros and not read.  The rows are
-// taken in the opposite order of the forward sweep: the ones it read last are still in L2.
+// Gradient of one row (or its split); rows without a coefficient are written as zeros and not read.  Taking the rows in
+// the opposite order of the forward sweep, with or without L2 policies that keep its last 32 MB, changed nothing
+// measurable (229 us against 228 for 4 x 256 pairs at 151936 columns).
 template <int THREADS, int UNROLL, bool CAP, bool SCALAR>
 __global__ void __launch_bounds__(THREADS) pref_dlogits_kernel(const Params p) {
-  const int64_t i = int64_t(gridDim.x) - 1 - blockIdx.x;
-  const int64_t r = i / p.splits;
-  const int k = int(i - r * p.splits);
+  const int64_t r = blockIdx.x / unsigned(p.splits);
+  const int k = int(blockIdx.x - r * p.splits);
   const int64_t b = r / p.seq_rows, t = r - b * p.seq_rows;
   const int64_t c0 = int64_t(k) * p.split_cols;
   const int64_t V = p.vocab - c0 < p.split_cols ? p.vocab - c0 : p.split_cols;
