@@ -37,7 +37,7 @@ __device__ __forceinline__ void put(__half* to, float v) { *to = __float2half_rn
 
 // 32 bytes at p + k, of which `n` (0, 16 or 32) are inside the row.
 template <bool WIDE>
-__device__ __forceinline__ void load32(uint32_t (&v)[8], const uint8_t* p, int64_t k, int64_t n) {
+__device__ __forceinline__ void load32(uint32_t (&v)[8], const uint8_t* p, int k, int n) {
   if (WIDE && n >= 32) {
     asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
@@ -75,21 +75,21 @@ __global__ void __launch_bounds__(kRowsThreads, 3) few_rows_kernel(const Params 
     const float* sx0 = p.x_scales + token(2 * t) * p.k_blocks;
     const float* sx1 = p.x_scales + token(2 * t + 1) * p.k_blocks;
     const float* sw = p.w_scales + n0 / 128 * p.k_blocks;
-    const int64_t left = p.hidden - t * 32;  // bytes of a row from this lane's first on (a multiple of 16)
+    const int left = int(p.hidden) - t * 32;  // bytes of a row from this lane's first on (a multiple of 16)
     // one block per warp and step, the next DEPTH of them on their way
     uint32_t a[DEPTH][8], b[DEPTH][8];
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      const int64_t k = int64_t(part + d * KS) * 128;
+      const int k = (part + d * KS) * 128;
       load32<WIDE>(a[d], wa, k, left - k);
       load32<WIDE>(b[d], wb, k, left - k);
     }
-    for (int64_t kb0 = part; kb0 < p.k_blocks; kb0 += KS * DEPTH) {
+    for (int kb0 = part; kb0 < p.k_blocks; kb0 += KS * DEPTH) {
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
-        const int64_t kb = kb0 + d * KS;
+        const int kb = kb0 + d * KS;
         if (kb >= p.k_blocks) break;
-        const int64_t k = kb * 128, next = k + int64_t(DEPTH * KS) * 128;
+        const int k = kb * 128, next = k + DEPTH * KS * 128;
         const float s = __ldg(sw + kb);
         float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll

@@ -787,7 +787,7 @@ int mllm_lm_head_fp8_matmul(const mllm_lm_head_fp8_args* a, void* stream) {
   if (!fp8::aligned(a->out, es)) return MLLM_GRPO_ERR_ALIGNMENT;
   p.out_aligned = fp8::aligned(a->out, 16) && (a->out_stride * es) % 16 == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->n_rows <= fp8::kFewRows) {
+  if (a->n_rows <= fp8::kFewRows && a->hidden_dim < (int64_t(1) << 30)) {  // it counts bytes of a row in 32 bits
     const cudaError_t e = fp8::launch_few_rows(p, a->out_dtype, s);
     return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);
   }
