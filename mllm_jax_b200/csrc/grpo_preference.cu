@@ -23,8 +23,10 @@ namespace pref {
 constexpr int kMaxSplits = 32;
 constexpr int64_t kTargetCtas = 4736;   // 32 per SM, about half of which have a masked row and leave
 constexpr int64_t kMinSplitCols = 8192; // 16 KB of a row per CTA at least
-constexpr int kPairThreads = 512;
-constexpr int64_t kOneCtaTokens = 16384;
+// Threads per pair, for answers of more than kShortTokens and for short ones (8192 pairs of single tokens: 62 us with
+// 512, 17 with 128; 8 pairs of 1024: 6.1 and 8.1; one pair of 16384: 25 and 82).
+constexpr int kPairThreads = 512, kPairThreadsShort = 128;
+constexpr int64_t kShortTokens = 128;
 
 struct Params {
   int64_t n_pairs, seq_rows, scored_rows, vocab, row_stride;
@@ -326,10 +328,11 @@ __device__ __forceinline__ void reduce_loss(const Params& p, double* red) {
 
 // One CTA per pair, half of it per answer.  From logits the CTA that finishes last adds the pairs up (the ticket was
 // zeroed by the stats launch before this one); from log-probs the sum has a launch of its own, since nothing ran before
-// to zero it.
-template <bool LOGPS>
-__global__ void __launch_bounds__(kPairThreads) pref_pairs_kernel(const Params p) {
-  constexpr int kHalf = kPairThreads / 2, kHalfWarps = kHalf / 32;
+// to zero it (5 us for both, up to a few hundred pairs; one CTA that does everything took 8.6 us for 8 pairs of 255
+// tokens and 49 for 256 pairs of one).
+template <bool LOGPS, int THREADS>
+__global__ void __launch_bounds__(THREADS) pref_pairs_kernel(const Params p) {
+  constexpr int kHalf = THREADS / 2, kHalfWarps = kHalf / 32;
   __shared__ double red[32];
   __shared__ SeqSums sums[2 * kHalfWarps];
   __shared__ float2 k_shared;
@@ -363,43 +366,6 @@ __global__ void __launch_bounds__(kPairThreads) pref_pairs_kernel(const Params p
     reduce_loss(p, red);
     if (threadIdx.x == 0 && p.call_status) *p.call_status = int32_t(atomicOr(p.ticket + 1, 0u));
   }
-}
-
-// Few tokens: one CTA, loss included.  A sequence has 32 / sequences warps (one at least).
-__global__ void __launch_bounds__(1024) pref_logps_one_cta_kernel(const Params p, const int warps_per_seq) {
-  __shared__ double red[32];
-  __shared__ SeqSums sums[32];
-  __shared__ float coef[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int at_once = 32 / warps_per_seq;  // sequences, an even number: chosen answers first, then the same pairs' rejected
-  const int half = at_once / 2, slot = warp / warps_per_seq, sub = warp % warps_per_seq;
-  for (int64_t pair0 = 0; pair0 < p.n_pairs; pair0 += half) {
-    const int64_t pair = pair0 + slot % half, s = pair + (slot / half) * p.n_pairs;
-    const bool in = pair < p.n_pairs;
-    SeqSums mine{0.0, 0.0, 0.0};
-    if (in) mine = warp_add(sequence_sums<true>(p, s, sub * 32 + lane, warps_per_seq * 32));
-    if (lane == 0) sums[warp] = mine;
-    __syncthreads();
-    if (threadIdx.x < half && pair0 + threadIdx.x < p.n_pairs) {
-      SeqSums a[2];
-      for (int k = 0; k < 2; ++k) {
-        const SeqSums* q = sums + (k * half + threadIdx.x) * warps_per_seq;
-        a[k] = q[0];
-        for (int w = 1; w < warps_per_seq; ++w) {
-          a[k].diff += q[w].diff;
-          a[k].lp += q[w].lp;
-          a[k].count += q[w].count;
-        }
-      }
-      const float2 k = finish_pair(p, pair0 + threadIdx.x, a[0], a[1]);
-      coef[threadIdx.x] = k.x;
-      coef[half + threadIdx.x] = k.y;
-    }
-    __syncthreads();
-    if (in && p.dlogps) write_dlogps(p, s, coef[slot], sub * 32 + lane, warps_per_seq * 32);
-  }
-  __syncthreads();
-  reduce_loss(p, red);
 }
 
 __global__ void __launch_bounds__(kPairThreads) pref_loss_kernel(const Params p) {
@@ -456,6 +422,15 @@ static cudaError_t done() {
   return cudaGetLastError();
 }
 
+template <bool LOGPS>
+static cudaError_t launch_pairs(const Params& p, cudaStream_t s) {
+  if (p.scored_rows <= kShortTokens)
+    pref_pairs_kernel<LOGPS, kPairThreadsShort><<<unsigned(p.n_pairs), kPairThreadsShort, 0, s>>>(p);
+  else
+    pref_pairs_kernel<LOGPS, kPairThreads><<<unsigned(p.n_pairs), kPairThreads, 0, s>>>(p);
+  return done();
+}
+
 static cudaError_t launch_forward(const Params& p, cudaStream_t s) {
   const unsigned grid = unsigned(2 * p.n_pairs * p.scored_rows * p.splits);
   const bool cap = p.softcap > 0.f, small = p.split_cols <= 16384;
@@ -471,8 +446,7 @@ static cudaError_t launch_forward(const Params& p, cudaStream_t s) {
   }
   cudaError_t e = done();
   if (e != cudaSuccess) return e;
-  pref_pairs_kernel<false><<<unsigned(p.n_pairs), kPairThreads, 0, s>>>(p);
-  return done();
+  return launch_pairs<false>(p, s);
 }
 
 template <bool CAP>
@@ -627,19 +601,10 @@ int mllm_grpo_preference_logps(const mllm_grpo_preference_args* args, void* stre
   const int st = pref::bind(args, pref::kLogps | pref::kForward, &p);
   if (st) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e;
-  if (2 * p.n_pairs * p.scored_rows <= pref::kOneCtaTokens) {
-    int per = 1;  // warps per sequence: 16 for one pair
-    while (per < 16 && per * 2 * 2 * p.n_pairs <= 32) per *= 2;
-    pref::pref_logps_one_cta_kernel<<<1, 1024, 0, s>>>(p, per);
+  cudaError_t e = pref::launch_pairs<true>(p, s);
+  if (e == cudaSuccess) {
+    pref::pref_loss_kernel<<<1, pref::kPairThreads, 0, s>>>(p);
     e = pref::done();
-  } else {
-    pref::pref_pairs_kernel<true><<<unsigned(p.n_pairs), pref::kPairThreads, 0, s>>>(p);
-    e = pref::done();
-    if (e == cudaSuccess) {
-      pref::pref_loss_kernel<<<1, pref::kPairThreads, 0, s>>>(p);
-      e = pref::done();
-    }
   }
   return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);
 }
