@@ -218,6 +218,23 @@ def call(name: str, args, stream: int) -> None:
                         lib.mllm_grpo_last_cuda_error().decode())
 
 
+def status_word(t, device) -> int:
+    """Address of a caller's MLLM_GRPO_DEV_* word."""
+    import torch
+
+    if t.device != device or t.dtype != torch.int32 or t.numel() != 1:
+        raise ValueError(f"device_status must be one int32 on {device}")
+    return t.data_ptr()
+
+
+def written(t) -> None:
+    """Tells autograd that a kernel has written a tensor of the caller's: what was saved of it is out of date."""
+    from torch.autograd.graph import increment_version
+
+    if not t.is_inference():
+        increment_version(t)
+
+
 def launch(name: str, args, device) -> None:
     """`call` on the current stream of `device` (a CUDA torch.device with an index), whichever device is current.
 

@@ -41,15 +41,13 @@ def _rows(t: torch.Tensor, hidden: int) -> torch.Tensor:
     return t if t.shape[0] == 0 or (t.stride(1) == 1 or hidden == 1) and t.stride(0) >= hidden else t.contiguous()
 
 
-def _args(n, vocab, hidden, scale, vocab_start, vocab_total, device_status) -> _lib.EmbeddingArgs:
+def _args(n, vocab, hidden, scale, vocab_start, vocab_total, device_status, dev) -> _lib.EmbeddingArgs:
     a = _lib.EmbeddingArgs()
     a.n_tokens, a.vocab, a.hidden = n, vocab, hidden
     a.vocab_start, a.vocab_total = int(vocab_start), 0 if vocab_total is None else int(vocab_total)
     a.scale = float(scale)
     if device_status is not None:
-        if not device_status.is_cuda or device_status.dtype != torch.int32 or device_status.numel() != 1:
-            raise ValueError("device_status must be one int32 on the device")
-        a.device_status = device_status.data_ptr()
+        a.device_status = _lib.status_word(device_status, dev)
     return a
 
 
@@ -58,7 +56,7 @@ def _lookup(ids, weight, scale, vocab_start, vocab_total, device_status) -> torc
     V, H = weight.shape
     ids32 = _ids(ids, dev)
     out = torch.empty(*ids.shape, H, dtype=weight.dtype, device=dev)
-    a = _args(ids32.numel(), V, H, scale, vocab_start, vocab_total, device_status)
+    a = _args(ids32.numel(), V, H, scale, vocab_start, vocab_total, device_status, dev)
     a.weight_stride, a.token_stride = max(weight.stride(0), H), H
     a.dtype = _dtype(weight, "weight")
     a.ids, a.weight, a.out = ids32.data_ptr(), weight.data_ptr(), out.data_ptr()
@@ -117,7 +115,7 @@ def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
     H = grad_out.shape[-1]
     g = _rows(grad_out, H)
     ids32 = _ids(ids, dev)
-    a = _args(ids32.numel(), vocab, H, scale, vocab_start, vocab_total, device_status)
+    a = _args(ids32.numel(), vocab, H, scale, vocab_start, vocab_total, device_status, dev)
     a.dtype = _dtype(grad_out, "grad_out")
     a.token_stride = max(g.stride(0), H) if g.shape[0] > 1 else H
     if out is None:
@@ -138,4 +136,6 @@ def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     a.ids, a.grad_out, a.dweight, a.workspace = ids32.data_ptr(), g.data_ptr(), res.data_ptr(), workspace.data_ptr()
     _lib.launch("mllm_grpo_embedding_grad", a, dev)
+    if out is not None:
+        _lib.written(out)
     return res

@@ -8,7 +8,7 @@ read, not trained.
 """
 from __future__ import annotations
 
-from typing import Tuple, Union
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -109,15 +109,17 @@ def _bind(x: Fp8Blocks, w: Fp8Blocks) -> _lib.Fp8Args:
 
 
 def fp8_matmul(x: Union[Fp8Blocks, torch.Tensor], w: Fp8Blocks, *, out_dtype: torch.dtype = torch.bfloat16,
-               out: torch.Tensor = None) -> torch.Tensor:
+               out: Optional[torch.Tensor] = None, device_status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [M, K] (Fp8Blocks with blocks of (1, 128), or a tensor, which is quantised first) times w [N, K] (blocks of
     (128, 128)), transposed: [M, N] of out_dtype (bf16, f16 or f32), rounded once.  K must be a multiple of 16.
-    `out` [M, N] (rows any distance apart) is written instead of a new tensor when given."""
+    `out` [M, N] (rows any distance apart) is written instead of a new tensor when given.  device_status (an int32 CUDA
+    tensor of the caller) has MLLM_GRPO_DEV_WAIT_TIMEOUT set if a wait inside the kernel ran out: the product is void."""
     if not isinstance(x, Fp8Blocks):
         x = quantize_fp8(x, block=(1, BLOCK))
     a = _bind(x, w)
     M, N = x.shape[0], w.shape[0]
-    if out is None:
+    given = out is not None
+    if not given:
         if out_dtype not in _DTYPES:
             raise TypeError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
         out = torch.empty(M, N, dtype=out_dtype, device=x.device)
@@ -125,5 +127,9 @@ def fp8_matmul(x: Union[Fp8Blocks, torch.Tensor], w: Fp8Blocks, *, out_dtype: to
             (out.stride(1) != 1 and N > 1) or (M > 1 and out.stride(0) < N):
         raise ValueError(f"out must be [{M}, {N}] of bfloat16, float16 or float32 on {x.device} with contiguous rows")
     a.out_stride, a.out_dtype, a.out = max(out.stride(0), N) if M > 1 else N, _DTYPES[out.dtype], out.data_ptr()
+    if device_status is not None:
+        a.device_status = _lib.status_word(device_status, x.device)
     _lib.launch("mllm_lm_head_fp8_matmul", a, x.device)
+    if given:
+        _lib.written(out)
     return out

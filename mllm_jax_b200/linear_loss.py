@@ -149,6 +149,8 @@ def _fp8_logprobs(a, hq: Fp8Blocks, weight: Fp8Blocks, token_ids, cfg: LossConfi
     vocabulary ranges and writes the results."""
     if token_ids.numel() != B * T:
         raise ValueError(f"chosen ids must have {B}x{T} elements, got shape {tuple(token_ids.shape)}")
+    if token_ids.dtype is torch.int64:
+        token_ids = token_ids.clamp(-1, 2 ** 31 - 1)  # an id beyond 32 bits must not wrap to a valid one
     ids = token_ids.to(device=dev, dtype=torch.int32).contiguous()
     status = torch.zeros(1, dtype=torch.int32, device=dev)
     out = torch.empty(3, B, T, dtype=torch.float32, device=dev)

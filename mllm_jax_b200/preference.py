@@ -116,7 +116,7 @@ class PreferenceProblem:
         """MLLM_GRPO_DEV_* bits of the forward from logits (an int32 on the device)."""
         return self.out[-1:].view(torch.int32)
 
-    def bind_logits(self, logits: torch.Tensor, ids: torch.Tensor, L: int) -> None:
+    def bind_logits(self, logits: torch.Tensor, ids: torch.Tensor, L: int, row_stride: int) -> None:
         self.logits = logits
         if ids.shape != (2 * self.P, self.T):
             raise ValueError(f"token ids must have {2 * self.P}x{self.T} elements, got shape {tuple(ids.shape)}")
@@ -124,7 +124,7 @@ class PreferenceProblem:
             ids = ids.clamp(-1, 2 ** 31 - 1)  # an id beyond 32 bits must not wrap to a valid one
         self.ids = _rows(ids, self.dev, (torch.int32,))
         a = self.a
-        a.seq_rows, a.vocab, a.row_stride = L, logits.shape[2], logits.stride(1)
+        a.seq_rows, a.vocab, a.row_stride = L, logits.shape[2], row_stride
         a.logits, a.chosen_ids, a.ids_stride = logits.data_ptr(), self.ids.data_ptr(), self.ids.stride(0)
 
     def bind_dlogits(self, dlogits: torch.Tensor) -> torch.Tensor:
@@ -153,13 +153,14 @@ def _from_logits(logits, token_ids, mask, ref, shifted, cfg, pair_weights, total
     if logits.dim() != 3:
         raise ValueError(f"logits must be [2P, L, V], got shape {tuple(logits.shape)}")
     B, L, V = logits.shape
-    if V < 1 or logits.stride(2) != 1 or logits.stride(1) < V or logits.stride(0) != L * logits.stride(1):
+    row = logits.stride(0) if L == 1 else logits.stride(1)
+    if V < 1 or (V > 1 and logits.stride(2) != 1) or row < V or logits.stride(0) != L * row:
         raise ValueError("logits must have unit stride on the vocabulary and rows evenly spaced")
     if shifted:
         token_ids, mask = token_ids[:, 1:], None if mask is None else mask[:, 1:]
     T = L - 1 if shifted else L
     prob = PreferenceProblem(B, T, logits.device, mask, ref, pair_weights, total_pairs, cfg or PreferenceConfig())
-    prob.bind_logits(logits, token_ids, L)
+    prob.bind_logits(logits, token_ids, L, row)
     return prob
 
 
@@ -184,6 +185,7 @@ def preference_value_and_grad(logits: torch.Tensor, token_ids: torch.Tensor, mas
                                                              device=logits.device)
     prob.bind_dlogits(dlogits)
     prob.run("mllm_grpo_preference_fwd_bwd")
+    _lib.written(dlogits)
     out = prob.outputs()
     out["dlogits"], out["problem"] = dlogits, prob
     return out
@@ -196,22 +198,25 @@ class _PreferenceLoss(torch.autograd.Function):
     def forward(ctx, logits, prob: PreferenceProblem, inplace_backward: bool):
         prob.run("mllm_grpo_preference_fwd")
         ctx.prob, ctx.inplace, ctx.spent = prob, inplace_backward, False
-        ctx.save_for_backward(logits)  # a change of the logits between the sweeps is an error
+        # a change of what the backward reads again, between the sweeps, is an error
+        ctx.save_for_backward(logits, prob.ids, *(() if prob.mask is None else (prob.mask,)))
         return prob.out[-2].clone()
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss):
         prob: PreferenceProblem = ctx.prob
-        (logits,) = ctx.saved_tensors
         if ctx.spent:
             raise RuntimeError("the first backward has overwritten the logits (inplace_backward=True)")
         ctx.spent = ctx.inplace
+        logits = ctx.saved_tensors[0]
         scale = grad_loss.to(torch.float32).reshape(1).contiguous()
         prob.a.grad_scale_dev = scale.data_ptr()
         prob.bind_dlogits(logits if ctx.inplace else torch.empty_strided(
             logits.shape, logits.stride(), dtype=logits.dtype, device=logits.device))
         prob.run("mllm_grpo_preference_bwd")
+        if ctx.inplace:
+            _lib.written(logits)  # another backward that needs what they held is an error
         return prob.dlogits, None, None
 
 

@@ -203,3 +203,35 @@ def test_streams_and_graph_replay(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[k][0]) and torch.equal(out[1], want[k][1])
+
+
+def test_sums_added_to_a_saved_tensor_are_seen(cuda):
+    """A gradient added into a tensor that autograd has saved makes that backward an error, not a wrong result."""
+    V, H = 40, 16
+    ids = torch.arange(5, device=cuda)
+    x = _rows(5, H, torch.float32, 11, cuda)
+    w = torch.ones(V, H, device=cuda, requires_grad=True)
+    buf = torch.zeros(V, H, device=cuda)
+    loss = (w * buf).sum()
+    G.embedding_grad(x, ids, V, out=buf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_captured_backward(cuda):
+    V, H = 70, 24
+    gen = torch.Generator().manual_seed(12)
+    ids = [torch.randint(0, V, (4, 30), generator=gen).to(cuda) for _ in range(2)]
+    c = _rows(120, H, torch.bfloat16, 12, cuda).reshape(4, 30, H)
+    want = [G.embedding_grad(c, i, V, scale=2.0, dtype=torch.bfloat16) for i in ids]
+    w = _rows(V, H, torch.bfloat16, 13, cuda).clone().requires_grad_(True)
+    static = ids[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        (grad,) = torch.autograd.grad(G.embedding_lookup(static, w, scale=2.0), w, c)
+    for k in (1, 0):
+        static.copy_(ids[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want[k])

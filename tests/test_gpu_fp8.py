@@ -247,3 +247,25 @@ def test_streams_and_graph_replay(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want[1])
+
+
+def test_product_reports_and_marks_what_it_writes(cuda):
+    x, w = _operands(20, 300, 256, 95, cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = torch.empty(20, 300, dtype=torch.bfloat16, device=cuda)
+    version = out._version
+    assert G.fp8_matmul(x, w, out=out, device_status=status) is out
+    assert out._version > version and int(status) == 0 and torch.equal(out, G.fp8_matmul(x, w))
+    with pytest.raises(ValueError, match="device_status"):
+        G.fp8_matmul(x, w, device_status=torch.zeros(1, dtype=torch.int32))
+
+
+def test_folded_head_clamps_ids_beyond_32_bits(cuda):
+    B, T, H, V = 1, 6, 64, 300
+    hidden = _x(T, H, torch.bfloat16, 96, cuda).view(B, T, H)
+    w = G.quantize_fp8(_x(V, H, torch.bfloat16, 97, cuda), block=(128, 128))
+    ids = torch.tensor([[0, 5, 2 ** 32 + 5, -(2 ** 32) + 5, V, V - 1]], device=cuda)
+    near = torch.tensor([[0, 5, V - 1, 0, V - 1, V - 1]], device=cuda)
+    out, want = lm_head_forward(hidden, w, ids), lm_head_forward(hidden, w, near)
+    assert torch.equal(out["per_token_logps"], want["per_token_logps"])
+    assert int(out["problem"].device_status) == 1 and int(want["problem"].device_status) == 0

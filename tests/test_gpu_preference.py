@@ -274,3 +274,72 @@ def test_streams_and_graph_replay(cuda):
         torch.cuda.synchronize()
         assert torch.equal(out["dlogits"], w["dlogits"]) and torch.equal(out["loss"], w["loss"])
         assert torch.equal(eager["dlogits"], w["dlogits"])
+
+
+@pytest.mark.parametrize("P,T", [(8192, 1), (600, 129), (3, 128), (64, 64)])
+def test_from_logps_many_or_short_pairs(cuda, P, T):
+    test_from_logps(cuda, P, T, "sigmoid", False)
+
+
+def test_single_rows_of_longer_sequences(cuda):
+    """L = 1 as a slice: the rows are the sequences' distance apart."""
+    logits, ids, mask, rf = _case(2, 5, 300, 30, cuda, prompt=False)
+    cfg = G.PreferenceConfig()
+    out = G.preference_value_and_grad(logits[:, 2:3], ids[:, 2:3], None, rf[:, 2:3], cfg=cfg)
+    _check(out, logits[:, 2:3], ids[:, 2:3], torch.ones_like(ids[:, 2:3]), rf[:, 2:3], cfg)
+    assert out["dlogits"].stride() == logits[:, 2:3].stride()
+
+
+@pytest.mark.parametrize("what", ["ids", "mask", "logits"])
+def test_a_change_between_the_sweeps_is_an_error(cuda, what):
+    logits, ids, mask, rf = _case(2, 9, 200, 31, cuda)
+    x = logits.clone().requires_grad_(True)
+    y = x * 1.0
+    out = G.preference_loss(y, ids, mask, rf[:, 1:])
+    if what == "logits":
+        with torch.no_grad():
+            y.mul_(2)
+    else:
+        dict(ids=ids, mask=mask)[what].zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out["loss"].backward()
+
+
+def test_gradients_written_over_the_logits_are_seen(cuda):
+    """Two losses of the same logits: once the first has written its gradient over them, the second cannot be formed."""
+    logits, ids, mask, rf = _case(2, 9, 200, 32, cuda)
+    x = logits.clone().requires_grad_(True)
+    y = x * 1.0
+    first = G.preference_loss(y, ids, mask, rf[:, 1:], inplace_backward=True)["loss"]
+    second = G.preference_loss(y, ids, mask, rf[:, 1:], cfg=G.PreferenceConfig(loss_type="ipo"))["loss"]
+    first.backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        second.backward()
+    z = logits.clone().requires_grad_(True)
+    w = z * 1.0
+    loss = G.preference_loss(w, ids, mask, rf[:, 1:])["loss"]
+    G.preference_value_and_grad(w.detach(), ids, mask, rf[:, 1:], shifted=True, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        G.preference_value_and_grad(logits * 1.0, ids, mask, rf[:, 1:], shifted=True, inplace=True)
+
+
+def test_captured_backward(cuda):
+    """Forward and backward of the differentiable forms in one graph, replayed with other logits."""
+    a, ids, mask, rf = _case(2, 9, 200, 33, cuda)
+    b = _case(2, 9, 200, 34, cuda)[0]
+    want = [G.preference_value_and_grad(t, ids, mask, rf[:, 1:], shifted=True) for t in (a, b)]
+    want = [(t["loss"].clone(), t["dlogits"].clone()) for t in want]
+    static = a.clone().requires_grad_(True)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        loss = G.preference_loss(static, ids, mask, rf[:, 1:])["loss"]
+        (grad,) = torch.autograd.grad(loss, static)
+    for k, t in ((1, b), (0, a)):
+        with torch.no_grad():
+            static.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(loss.detach(), want[k][0]) and torch.equal(grad, want[k][1])

@@ -221,3 +221,23 @@ def test_preference_arguments_are_checked(built_lib):
                        (dict(ref=torch.ones(2)), "ref_per_token_logps"), (dict(w=torch.ones(4)), "pair_weights")):
         with pytest.raises(ValueError, match=match):
             make(**bad)
+
+
+def test_status_words_are_checked():
+    from mllm_jax_b200 import _lib
+    cpu = torch.device("cpu")
+    word = torch.zeros(1, dtype=torch.int32)
+    assert _lib.status_word(word, cpu) == word.data_ptr()
+    for bad in (torch.zeros(1), torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32, device="meta")):
+        with pytest.raises(ValueError, match="device_status"):
+            _lib.status_word(bad, cpu)
+
+
+def test_written_tensors_change_their_version():
+    from mllm_jax_b200 import _lib
+    t = torch.zeros(3)
+    before = t._version
+    _lib.written(t[1:])
+    assert t._version > before
+    with torch.inference_mode():
+        _lib.written(torch.zeros(3))
