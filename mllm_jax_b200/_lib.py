@@ -212,7 +212,7 @@ def call(name: str, args, stream: int) -> None:
     """Invoke one launcher; raise GrpoError on a non-zero status."""
     lib = load()
     args.struct_size = C.sizeof(type(args))
-    status = getattr(lib, name)(C.byref(args), C.c_void_p(stream))
+    status = getattr(lib, name)(C.byref(args), stream)
     if status != 0:
         raise GrpoError(name, status, lib.mllm_grpo_status_string(status).decode(),
                         lib.mllm_grpo_last_cuda_error().decode())
@@ -240,16 +240,14 @@ def launch(name: str, args, device) -> None:
 
     A call of a few microseconds on the GPU is bound by the host: switching to a device that is already current and
     wrapping its stream in an object cost 8 us of the 25 us that a small lookup took."""
-    from torch._C import _cuda_getCurrentRawStream, _cuda_getDevice
+    import torch
 
-    index = device.index
-    if _cuda_getDevice() == index:
-        call(name, args, _cuda_getCurrentRawStream(index))
+    index, c = device.index, torch._C
+    if c._cuda_getDevice() == index:
+        call(name, args, c._cuda_getCurrentRawStream(index))
     else:
-        import torch
-
         with torch.cuda.device(index):
-            call(name, args, _cuda_getCurrentRawStream(index))
+            call(name, args, c._cuda_getCurrentRawStream(index))
 
 
 def launch_count() -> int:

@@ -6,11 +6,14 @@
 //
 // Gradient: the new [V, H] gradient has to be written whole (at V = 151936, H = 3584 that is 2.18 GB of f32 against
 // 0.23 GB of token gradients), nearly all of it zeros.  Its sums need the tokens grouped by id in an order that depends
-// on the ids alone: a stable radix sort of (id, token) pairs by ONE cluster of eight CTAs, whose digit counts meet in
-// distributed shared memory.  Then, in one launch, a few resident CTAs sum and write the rows that have tokens from a
-// list of them, and short CTAs fill the others with zeros, 32 KB each in the order of the addresses.  (CTAs that stay
-// resident and walk the table fill it at 6.1 TB/s, short ones in order at 7.5.  A loop over the table's rows that sums
-// where there are tokens holds the fill up: a load waits several microseconds behind the stores.)
+// on the ids alone: a stable radix sort of (id, token) pairs by ONE cluster of CTAs, whose digit counts meet in
+// distributed shared memory.  It leaves nearly all SMs idle, so the zeros are written beside it: their launch does not
+// wait for the sort's (programmatic launch), only its last CTA does before it leaves, and the rows that have tokens are
+// summed and written after both.  Where those rows are so many that writing them twice costs more than the sort
+// (rows_after_fill), zeros go only into the others, in the launch that sums: a few resident CTAs sum rows from a list and
+// short CTAs fill, 32 KB each in the order of the addresses.  (CTAs that stay resident and walk the table fill it at
+// 6.1 TB/s, short ones in order at 7.5.  A loop over the table's rows that sums where there are tokens holds the fill
+// up: a load waits several microseconds behind the stores.)
 // A row with very many tokens (padding, a frequent word) would keep one CTA busy long after all others: runs of 32
 // equal ids that start at a multiple of 32 in the sorted order are summed beforehand, and eight warps share what is left
 // of such a row.  Every sum is f32 in a fixed order.
@@ -110,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const LookupParams p) 
 
 // ---------------------------------------------------------------------------------------------
 // Stable radix sort of (id, token) by one cluster of eight CTAs (one CTA for up to 4096 pairs, 16 beyond 32768), 9 bits a
-// pass.  CTA r owns the r-th eighth of the pairs, in tiles of 4096, 128 consecutive pairs per warp.  Inside a tile a pair's place among
+// pass.  CTA r owns the r-th eighth (sixteenth) of the pairs, in tiles of 4096, 128 consecutive pairs per warp.  Inside a tile a pair's place among
 // its digit is found by the warp's match of equal digits (stable: lower lanes first) and the running counts of the warps
 // before it; all eight CTAs' digit counts through distributed shared memory give every digit its first place.  Two
 // passes: 12 us for up to 4096 pairs, 25 us for 32768.
@@ -155,6 +158,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) 
   __shared__ alignas(16) uint16_t count[kSortWarps][kBins];
   __shared__ uint32_t scan[kBins / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // zeros, if they come next, need not wait
   if (blockIdx.x >= CTAS) {  // whole clusters
     const int64_t words = (p.vocab + 15) / 16, step = int64_t(gridDim.x - CTAS) * kSortThreads;
     for (int64_t i = int64_t(blockIdx.x - CTAS) * kSortThreads + tid; i < words; i += step) p.busy[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -308,6 +312,7 @@ struct Lists {
 struct GradParams {
   int64_t grad_stride, weight_stride;
   uint32_t n, hidden, vocab, row_vecs, accumulate;
+  uint32_t filled;  // the zeros have been written
   uint32_t group;  // threads that share a light row: 32, 64, 128 or 256
   uint32_t parts;  // parts of 32 vectors of a row
   uint32_t row_ctas;
@@ -389,7 +394,7 @@ __global__ void __launch_bounds__(128) run_kernel(const GradParams p, const uint
       p.lists.heavy[hb + __popc(hs & lower)] = i;
     else if (head)
       p.lists.light[lb + __popc(ls & lower)] = Light{mine, i, count, 0u};
-    if (head && !p.accumulate) p.busy[mine] = 1;
+    if (head && !p.accumulate && !p.filled) p.busy[mine] = 1;
     return;
   }
   const uint32_t k = __shfl_sync(0xffffffffu, mine, 0);
@@ -553,6 +558,8 @@ __device__ __forceinline__ void fill(const FillParams& p, uint32_t block) {
 template <typename W>
 __global__ void __launch_bounds__(kThreads, 8) fill_kernel(const FillParams p) {
   fill<W>(p, blockIdx.x);
+  // beside the sort (rows_after_fill): this launch ends after the sort does, whatever comes next finds both complete
+  if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // CTAs [0, p.row_ctas) sum the rows that have tokens; the others fill.
@@ -651,12 +658,21 @@ static FillParams fill_params(const mllm_grpo_embedding_args* a, const uint8_t* 
 static unsigned fill_ctas(const FillParams& f) { return (f.total + kThreads * kVecs - 1) / (kThreads * kVecs); }
 
 template <typename W>
-static cudaError_t launch_fill(const mllm_grpo_embedding_args* a, const uint8_t* busy, int64_t from, cudaStream_t s) {
+static cudaError_t launch_fill(const mllm_grpo_embedding_args* a, const uint8_t* busy, int64_t from, bool beside, cudaStream_t s) {
   const int64_t rows_per = kMostWords / (a->hidden * elem(a->out_dtype) / int64_t(sizeof(W)));
   for (int64_t r0 = from; r0 < a->vocab; r0 += rows_per) {
     const FillParams f = fill_params<W>(a, busy, r0, a->vocab - r0 < rows_per ? a->vocab - r0 : rows_per);
-    fill_kernel<W><<<fill_ctas(f), kThreads, 0, s>>>(f);
-    const cudaError_t e = done();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(fill_ctas(f));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = beside && r0 == from ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fill_kernel<W>, f);
+    count_launch();
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -667,7 +683,7 @@ static cudaError_t launch_rows_w(const mllm_grpo_embedding_args* a, GradParams p
   // four CTAs are resident per SM: with many rows they are all busy with rows at first
   const int64_t most = 148 * 4, items = (int64_t(p.n) * p.group + kThreads - 1) / kThreads;
   p.row_ctas = uint32_t(items < most ? items : most);
-  if (a->accumulate) {
+  if (a->accumulate || p.filled) {
     grad_rows_kernel<T, O, EV, W><<<p.row_ctas, kThreads, 0, s>>>(p, FillParams{0, 0, 1, FastDiv(1), nullptr, nullptr});
     return done();
   }
@@ -676,13 +692,29 @@ static cudaError_t launch_rows_w(const mllm_grpo_embedding_args* a, GradParams p
   const FillParams f = fill_params<W>(a, p.busy, 0, rows);
   grad_rows_kernel<T, O, EV, W><<<p.row_ctas + fill_ctas(f), kThreads, 0, s>>>(p, f);
   const cudaError_t e = done();
-  return e == cudaSuccess ? launch_fill<W>(a, p.busy, rows, s) : e;
+  return e == cudaSuccess ? launch_fill<W>(a, p.busy, rows, false, s) : e;
 }
 
 // Zeros are written in the widest words that every row allows: 16 bytes, or an element.
 static bool wide_rows(const mllm_grpo_embedding_args* a) {
   const int64_t eo = elem(a->out_dtype);
   return ((a->hidden * eo | a->weight_stride * eo | int64_t(reinterpret_cast<uintptr_t>(a->dweight) & 15)) & 15) == 0;
+}
+
+// The whole gradient's zeros.
+static cudaError_t launch_zeros(const mllm_grpo_embedding_args* a, bool beside, cudaStream_t s) {
+  if (wide_rows(a)) return launch_fill<uint4>(a, nullptr, 0, beside, s);
+  return a->out_dtype == MLLM_GRPO_F32 ? launch_fill<uint32_t>(a, nullptr, 0, beside, s)
+                                       : launch_fill<uint16_t>(a, nullptr, 0, beside, s);
+}
+
+// Whether the zeros of the whole gradient are written beside the sort, and the rows that have tokens after that: these
+// are then written twice, which costs less than the sort where they are few or narrow.  151936 f32 rows, this way / with
+// the zeros in the last launch: 2048 tokens of width 896 84 / 94 us, 32768 of them 127 / 135, 4096 of width 3584
+// 322 / 328; but 8192 of width 3584 346 / 335, 16384 of them 390 / 366.
+static bool rows_after_fill(const mllm_grpo_embedding_args* a) {
+  const int64_t row = a->hidden * elem(a->out_dtype);
+  return !a->accumulate && (row <= 4096 || a->n_tokens * row <= int64_t(64) << 20);
 }
 
 template <typename T, typename O, int EV>
@@ -838,10 +870,12 @@ int mllm_grpo_embedding_grad(const mllm_grpo_embedding_args* a, void* stream) {
   const int last = (q.passes - 1) & 1;
   cudaError_t e = cudaSuccess;
   if (n) {
-    e = emb::launch_sort(q, a->accumulate == 0, s);
+    const bool filled = emb::rows_after_fill(a);
+    e = emb::launch_sort(q, !a->accumulate && !filled, s);
+    if (e == cudaSuccess && filled) e = emb::launch_zeros(a, true, s);
     if (e != cudaSuccess) return record_cuda_error(e);
     emb::GradParams p{a->token_stride, a->weight_stride, n, uint32_t(a->hidden), uint32_t(a->vocab), 0, a->accumulate ? 1u : 0u,
-                      0, 0, 0, emb::FastDiv(1), a->scale, q.key[last], q.idx[last], reinterpret_cast<uint8_t*>(q.busy), lists,
+                      filled ? 1u : 0u, 0, 0, 0, emb::FastDiv(1), a->scale, q.key[last], q.idx[last], reinterpret_cast<uint8_t*>(q.busy), lists,
                       a->grad_out, a->dweight,
                       reinterpret_cast<float*>(w + list + 16 + int64_t(n) * int64_t(sizeof(emb::Light)))};
     if (a->dtype == MLLM_GRPO_BF16)
@@ -851,14 +885,7 @@ int mllm_grpo_embedding_grad(const mllm_grpo_embedding_args* a, void* stream) {
     else
       e = emb::launch_grad_t<float>(a, p, s);
   }
-  if (n == 0) {  // all zeros (the accumulated form has returned)
-    if (emb::wide_rows(a))
-      e = emb::launch_fill<uint4>(a, nullptr, 0, s);
-    else if (a->out_dtype == MLLM_GRPO_F32)
-      e = emb::launch_fill<uint32_t>(a, nullptr, 0, s);
-    else
-      e = emb::launch_fill<uint16_t>(a, nullptr, 0, s);
-  }
+  if (n == 0) e = emb::launch_zeros(a, false, s);  // the accumulated form has returned
   return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);
 }
 

@@ -140,8 +140,9 @@ class PreferenceProblem:
         _lib.launch(entry, self.a, self.dev)
 
     def outputs(self) -> dict:
-        good, bad, good_lp, bad_lp, rest = self.out.split((self.P, self.P, self.P, self.P, 2))
-        return {"loss": rest[0], "chosen_rewards": good, "rejected_rewards": bad, "chosen_logps": good_lp,
+        P = self.P
+        good, bad, good_lp, bad_lp, _ = self.out.split_with_sizes((P, P, P, P, 2))
+        return {"loss": self.out.select(0, -2), "chosen_rewards": good, "rejected_rewards": bad, "chosen_logps": good_lp,
                 "rejected_logps": bad_lp}
 
 
@@ -180,12 +181,14 @@ def preference_value_and_grad(logits: torch.Tensor, token_ids: torch.Tensor, mas
     [P], dlogits and the problem (whose device_status has MLLM_GRPO_DEV_ID_CLAMPED for ids outside the vocabulary)."""
     prob = _from_logits(logits, token_ids, mask, ref_per_token_logps, shifted, cfg, pair_weights, total_pairs)
     prob.a.grad_scale = float(grad_scale)
+    given = inplace or dlogits is not None
     if dlogits is None:
         dlogits = logits if inplace else torch.empty_strided(logits.shape, logits.stride(), dtype=logits.dtype,
                                                              device=logits.device)
     prob.bind_dlogits(dlogits)
     prob.run("mllm_grpo_preference_fwd_bwd")
-    _lib.written(dlogits)
+    if given:
+        _lib.written(dlogits)
     out = prob.outputs()
     out["dlogits"], out["problem"] = dlogits, prob
     return out
@@ -200,7 +203,7 @@ class _PreferenceLoss(torch.autograd.Function):
         ctx.prob, ctx.inplace, ctx.spent = prob, inplace_backward, False
         # a change of what the backward reads again, between the sweeps, is an error
         ctx.save_for_backward(logits, prob.ids, *(() if prob.mask is None else (prob.mask,)))
-        return prob.out[-2].clone()
+        return prob.out.select(0, -2).clone()
 
     @staticmethod
     @once_differentiable
@@ -246,7 +249,7 @@ def preference_logps_value_and_grad(per_token_logps: torch.Tensor, mask: Optiona
         raise ValueError(f"per_token_logps must be [2P, T], got shape {tuple(x.shape)}")
     prob = PreferenceProblem(x.shape[0], x.shape[1], x.device, mask, ref_per_token_logps, pair_weights, total_pairs,
                              cfg or PreferenceConfig())
-    prob.logps = _f32(x.detach(), x.device, (x.shape,), "per_token_logps")
+    prob.logps = _f32(x.detach() if x.requires_grad else x, x.device, (x.shape,), "per_token_logps")
     dlogps = torch.empty_like(prob.logps)
     prob.a.token_logps, prob.a.dtoken_logps = prob.logps.data_ptr(), dlogps.data_ptr()
     prob.a.grad_scale = float(grad_scale)
