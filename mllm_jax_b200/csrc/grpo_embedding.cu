@@ -7,13 +7,14 @@
 // Gradient: the new [V, H] gradient has to be written whole (at V = 151936, H = 3584 that is 2.18 GB of f32 against
 // 0.23 GB of token gradients), nearly all of it zeros.  Its sums need the tokens grouped by id in an order that depends
 // on the ids alone: a stable radix sort of (id, token) pairs by ONE cluster of CTAs, whose digit counts meet in
-// distributed shared memory.  It leaves nearly all SMs idle, so the zeros are written beside it: their launch does not
-// wait for the sort's (programmatic launch), only its last CTA does before it leaves, and the rows that have tokens are
-// summed and written after both.  Where those rows are so many that writing them twice costs more than the sort
-// (rows_after_fill), zeros go only into the others, in the launch that sums: a few resident CTAs sum rows from a list and
-// short CTAs fill, 32 KB each in the order of the addresses.  (CTAs that stay resident and walk the table fill it at
-// 6.1 TB/s, short ones in order at 7.5.  A loop over the table's rows that sums where there are tokens holds the fill
-// up: a load waits several microseconds behind the stores.)
+// distributed shared memory.  It leaves nearly all SMs idle, so zeros are written beside it: their launch does not wait
+// for the sort's (programmatic launch), only CTAs late in it do, which then list the rows that have tokens.  A last launch
+// sums and writes those, after the zeros.  Where the rows with tokens are so many that writing them twice costs more than
+// the sort (rows_beside), only the first part of the table gets its zeros early, and the last launch fills the rest where
+// there are no tokens: a few resident CTAs sum rows from the list and short CTAs fill, 32 KB each in the order of the
+// addresses.  (CTAs that stay resident and walk the table fill it at 6.1 TB/s, short ones in order at 7.5.  A loop over
+// the table's rows that sums where there are tokens holds the fill up: a load waits several microseconds behind the
+// stores.)
 // A row with very many tokens (padding, a frequent word) would keep one CTA busy long after all others: runs of 32
 // equal ids that start at a multiple of 32 in the sorted order are summed beforehand, and eight warps share what is left
 // of such a row.  Every sum is f32 in a fixed order.
@@ -21,6 +22,7 @@
 
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "grpo_cluster.cuh"
 #include "grpo_common.cuh"
@@ -116,7 +118,7 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const LookupParams p) 
 // pass.  CTA r owns the r-th eighth (sixteenth) of the pairs, in tiles of 4096, 128 consecutive pairs per warp.  Inside a tile a pair's place among
 // its digit is found by the warp's match of equal digits (stable: lower lanes first) and the running counts of the warps
 // before it; all eight CTAs' digit counts through distributed shared memory give every digit its first place.  Two
-// passes: 12 us for up to 4096 pairs, 25 us for 32768.
+// passes: 14 us for up to 4096 pairs, 25 us for 32768.
 // ---------------------------------------------------------------------------------------------
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
@@ -289,6 +291,42 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) 
   }
 }
 
+// Zeros in the rows without tokens, kVecs words W a thread in the order of their addresses.
+constexpr int kVecs = 8;
+struct FillParams {
+  int64_t stride;  // of a row, in words
+  uint32_t total;  // words of this launch's rows
+  uint32_t row_words;
+  FastDiv by_row;
+  const uint8_t* busy;  // of this launch's rows; null: no row has tokens
+  void* out;
+};
+template <typename W>
+__device__ __forceinline__ void fill(const FillParams& p, uint32_t block) {
+  const uint32_t base = block * uint32_t(kThreads * kVecs) + threadIdx.x;
+  uint32_t skip = 0;
+  if (p.busy) {
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const uint32_t i = base + u * kThreads;
+      if (i < p.total && p.busy[p.by_row.div(i)]) skip |= 1u << u;
+    }
+  }
+  W zero;
+  memset(&zero, 0, sizeof(W));
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const uint32_t i = base + u * kThreads;
+    if (i >= p.total || (skip >> u & 1u)) continue;
+    const uint32_t r = p.by_row.div(i);
+    static_cast<W*>(p.out)[r * p.stride + (i - r * p.row_words)] = zero;
+  }
+}
+template <typename W>
+__global__ void __launch_bounds__(kThreads, 8) fill_kernel(const FillParams p) {
+  fill<W>(p, blockIdx.x);
+}
+
 // ---------------------------------------------------------------------------------------------
 // Sums
 // ---------------------------------------------------------------------------------------------
@@ -312,7 +350,7 @@ struct Lists {
 struct GradParams {
   int64_t grad_stride, weight_stride;
   uint32_t n, hidden, vocab, row_vecs, accumulate;
-  uint32_t filled;  // the zeros have been written
+  uint32_t filled;  // rows below this one have their zeros already (all of them where the gradient is accumulated)
   uint32_t group;  // threads that share a light row: 32, 64, 128 or 256
   uint32_t parts;  // parts of 32 vectors of a row
   uint32_t row_ctas;
@@ -366,40 +404,41 @@ __device__ __forceinline__ void store_vec(O* to, const float (&acc)[EV], float s
   }
 }
 
-// Lists and marks the rows that have tokens (CTAs of their own), and sums runs of 32 equal ids, 8 token rows of 16
-// bytes a thread (16 of 8 or fewer) on the way at a time.  blockIdx.x = 32 sorted places, blockIdx.y = part of the columns.
+// Lists and marks the rows that have tokens: one warp per 32 sorted places.
+__device__ __forceinline__ void list_rows(const GradParams& p, uint32_t block) {
+  const uint32_t lane = threadIdx.x & 31, i = block * kRun + lane;
+  const uint32_t mine = i < p.n ? p.key[i] : 0xffffffffu;
+  const uint32_t before = i > 0 && i < p.n ? p.key[i - 1] : 0xffffffffu;
+  const uint32_t after = i + kRun < p.n ? p.key[i + kRun] : 0xffffffffu;  // the next 32 places
+  const bool head = mine < p.vocab && (i == 0 || before != mine);
+  // how many tokens the row has (up to 64 are seen from here): equal keys are neighbours
+  const uint32_t last = __shfl_sync(0xffffffffu, mine, 31);
+  const uint32_t over = __popc(__ballot_sync(0xffffffffu, after == last));
+  const uint32_t count = __popc(__match_any_sync(0xffffffffu, mine)) + (mine == last ? over : 0u);
+  const bool heavy = head && count > kLight;
+  const uint32_t lower = (1u << lane) - 1u;
+  const uint32_t hs = __ballot_sync(0xffffffffu, heavy), ls = __ballot_sync(0xffffffffu, head && !heavy);
+  uint32_t at = 0;
+  if (lane == 0 && ls) at = atomicAdd(p.lists.counts, uint32_t(__popc(ls)));
+  if (lane == 1 && hs) at = atomicAdd(p.lists.counts + 1, uint32_t(__popc(hs)));
+  const uint32_t lb = __shfl_sync(0xffffffffu, at, 0), hb = __shfl_sync(0xffffffffu, at, 1);
+  if (heavy)
+    p.lists.heavy[hb + __popc(hs & lower)] = i;
+  else if (head)
+    p.lists.light[lb + __popc(ls & lower)] = Light{mine, i, count, 0u};
+  if (head && mine >= p.filled) p.busy[mine] = 1;
+}
+
+// Sums 32 places whose ids are all equal, EV columns a thread (c is this thread's vector of them), 8 token rows of 16
+// bytes a thread (16 of 8 or fewer) on the way at a time.
 template <typename T, int EV>
-__global__ void __launch_bounds__(128) run_kernel(const GradParams p, const uint32_t row_vecs) {
+__device__ __forceinline__ void sum_run(const GradParams& p, uint32_t block, uint32_t c, uint32_t row_vecs) {
   constexpr uint32_t B = EV * sizeof(T) == 16 ? 8 : 16;
-  const uint32_t lane = threadIdx.x & 31, i = blockIdx.x * kRun + lane;
+  const uint32_t i = block * kRun + (threadIdx.x & 31);
   const uint32_t mine = i < p.n ? p.key[i] : 0xffffffffu;
   const uint32_t tokens = i < p.n ? p.idx[i] : 0u;
-  if (blockIdx.y == gridDim.y - 1) {  // the last one has no columns: it lists and marks
-    if (threadIdx.x >= 32) return;
-    const uint32_t before = i > 0 && i < p.n ? p.key[i - 1] : 0xffffffffu;
-    const uint32_t after = i + kRun < p.n ? p.key[i + kRun] : 0xffffffffu;  // the next 32 places
-    const bool head = mine < p.vocab && (i == 0 || before != mine);
-    // how many tokens the row has (up to 64 are seen from here): equal keys are neighbours
-    const uint32_t last = __shfl_sync(0xffffffffu, mine, 31);
-    const uint32_t over = __popc(__ballot_sync(0xffffffffu, after == last));
-    const uint32_t count = __popc(__match_any_sync(0xffffffffu, mine)) + (mine == last ? over : 0u);
-    const bool heavy = head && count > kLight;
-    const uint32_t lower = (1u << lane) - 1u;
-    const uint32_t hs = __ballot_sync(0xffffffffu, heavy), ls = __ballot_sync(0xffffffffu, head && !heavy);
-    uint32_t at = 0;
-    if (lane == 0 && ls) at = atomicAdd(p.lists.counts, uint32_t(__popc(ls)));
-    if (lane == 1 && hs) at = atomicAdd(p.lists.counts + 1, uint32_t(__popc(hs)));
-    const uint32_t lb = __shfl_sync(0xffffffffu, at, 0), hb = __shfl_sync(0xffffffffu, at, 1);
-    if (heavy)
-      p.lists.heavy[hb + __popc(hs & lower)] = i;
-    else if (head)
-      p.lists.light[lb + __popc(ls & lower)] = Light{mine, i, count, 0u};
-    if (head && !p.accumulate && !p.filled) p.busy[mine] = 1;
-    return;
-  }
   const uint32_t k = __shfl_sync(0xffffffffu, mine, 0);
   if (__shfl_sync(0xffffffffu, mine, 31) != k || k >= p.vocab) return;
-  const uint32_t c = blockIdx.y * blockDim.x + threadIdx.x;
   const bool ok = c < row_vecs;
   float acc[EV] = {};
 #pragma unroll
@@ -414,8 +453,46 @@ __global__ void __launch_bounds__(128) run_kernel(const GradParams p, const uint
     for (uint32_t j = 0; j < B; ++j)
       if (ok) add_vec<T, EV>(acc, x[j]);
   }
-  if (ok) store_vec<float, EV>(p.run + int64_t(blockIdx.x) * p.hidden + int64_t(c) * EV, acc, 1.0f);
+  if (ok) store_vec<float, EV>(p.run + int64_t(block) * p.hidden + int64_t(c) * EV, acc, 1.0f);
 }
+
+// blockIdx.x = 32 sorted places, blockIdx.y = part of the columns, the last one the list.
+template <typename T, int EV>
+__global__ void __launch_bounds__(128) run_kernel(const GradParams p, const uint32_t row_vecs) {
+  if (blockIdx.y == gridDim.y - 1) {
+    if (threadIdx.x < 32) list_rows(p, blockIdx.x);
+    return;
+  }
+  sum_run<T, EV>(p, blockIdx.x, blockIdx.y * blockDim.x + threadIdx.x, row_vecs);
+}
+
+// The same beside the zeros: CTAs [first, first + list_ctas + sum_ctas) wait for the sort to be complete, then list rows
+// and sum runs, the others fill.
+struct Beside {
+  uint32_t row_vecs, parts;  // vectors of a row; warps that share one run
+  uint32_t first, list_ctas, sum_ctas;
+};
+template <typename T, int EV, typename W>
+__global__ void __launch_bounds__(kThreads, 3) fill_runs_kernel(const GradParams p, const FillParams f, const Beside b) {
+  if (blockIdx.x < b.first) {
+    fill<W>(f, blockIdx.x);
+    return;
+  }
+  const uint32_t at = blockIdx.x - b.first, warps = kThreads / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (at >= b.list_ctas + b.sum_ctas) {
+    fill<W>(f, blockIdx.x - b.list_ctas - b.sum_ctas);
+    return;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint32_t runs = (p.n + kRun - 1) / kRun;
+  if (at < b.list_ctas) {
+    if (at * warps + warp < runs) list_rows(p, at * warps + warp);
+    return;
+  }
+  const uint32_t item = (at - b.list_ctas) * warps + warp, run = item / b.parts;
+  if (run < runs) sum_run<T, EV>(p, run, (item - run * b.parts) * 32 + lane, b.row_vecs);
+}
+
 // First place in [lo, hi) whose key is >= v, found by a whole warp (32 probes a step).
 __device__ __forceinline__ uint32_t warp_lower_bound(const uint32_t* key, uint32_t lo, uint32_t hi, uint64_t v) {
   const uint32_t lane = threadIdx.x & 31;
@@ -450,7 +527,7 @@ template <typename T, typename O, int EV>
 __device__ __forceinline__ void heavy_rows(const GradParams& p, float (&meet)[kSumWarps][32][EV]) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t items = p.lists.counts[1] * p.parts;
-  for (uint32_t item = blockIdx.x; item < items; item += p.row_ctas) {
+  for (uint32_t item = p.row_ctas - 1 - blockIdx.x; item < items; item += p.row_ctas) {  // the last CTAs have the fewest light rows
     const uint32_t r = p.by_part.div(item), c = (item - r * p.parts) * 32 + lane;
     const bool ok = c < p.row_vecs;
     const uint32_t s = p.lists.heavy[r], k = p.key[s];
@@ -524,44 +601,6 @@ __device__ __forceinline__ void light_rows(const GradParams& p) {
   }
 }
 
-// Zeros in the rows without tokens, kVecs words W a thread in the order of their addresses.
-constexpr int kVecs = 8;
-struct FillParams {
-  int64_t stride;  // of a row, in words
-  uint32_t total;  // words of this launch's rows
-  uint32_t row_words;
-  FastDiv by_row;
-  const uint8_t* busy;  // of this launch's rows; null: no row has tokens
-  void* out;
-};
-template <typename W>
-__device__ __forceinline__ void fill(const FillParams& p, uint32_t block) {
-  const uint32_t base = block * uint32_t(kThreads * kVecs) + threadIdx.x;
-  uint32_t skip = 0;
-  if (p.busy) {
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      const uint32_t i = base + u * kThreads;
-      if (i < p.total && p.busy[p.by_row.div(i)]) skip |= 1u << u;
-    }
-  }
-  W zero;
-  memset(&zero, 0, sizeof(W));
-#pragma unroll
-  for (int u = 0; u < kVecs; ++u) {
-    const uint32_t i = base + u * kThreads;
-    if (i >= p.total || (skip >> u & 1u)) continue;
-    const uint32_t r = p.by_row.div(i);
-    static_cast<W*>(p.out)[r * p.stride + (i - r * p.row_words)] = zero;
-  }
-}
-template <typename W>
-__global__ void __launch_bounds__(kThreads, 8) fill_kernel(const FillParams p) {
-  fill<W>(p, blockIdx.x);
-  // beside the sort (rows_after_fill): this launch ends after the sort does, whatever comes next finds both complete
-  if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 // CTAs [0, p.row_ctas) sum the rows that have tokens; the others fill.
 template <typename T, typename O, int EV, typename W>
 __global__ void __launch_bounds__(kThreads, 4) grad_rows_kernel(const GradParams p, const FillParams f) {
@@ -629,21 +668,6 @@ static cudaError_t launch_lookup_t(const mllm_grpo_embedding_args* a, LookupPara
   return cudaSuccess;
 }
 
-template <typename T, int EV>
-static cudaError_t launch_runs(const GradParams& p, cudaStream_t s) {
-  const uint32_t runs = (p.n + kRun - 1) / kRun;
-  const auto go = [&](auto* kernel, uint32_t row_vecs) {
-    const uint32_t threads = row_vecs <= 32 ? 32 : (row_vecs <= 64 ? 64 : 128);
-    kernel<<<dim3(runs, (row_vecs + threads - 1) / threads + 1), threads, 0, s>>>(p, row_vecs);
-  };
-  constexpr int kWide = 16 / int(sizeof(T));
-  if (vec_of(p.hidden, kWide, p.grad, p.grad_stride, sizeof(T), p.run, p.hidden, 2) == kWide)
-    go(run_kernel<T, kWide>, p.hidden / kWide);
-  else
-    go(run_kernel<T, EV>, p.row_vecs);
-  return done();
-}
-
 constexpr int64_t kMostWords = int64_t(1) << 31;  // words are counted in 32 bits
 
 // The rows [r0, r0 + rows) of the gradient in words of W.
@@ -658,24 +682,49 @@ static FillParams fill_params(const mllm_grpo_embedding_args* a, const uint8_t* 
 static unsigned fill_ctas(const FillParams& f) { return (f.total + kThreads * kVecs - 1) / (kThreads * kVecs); }
 
 template <typename W>
-static cudaError_t launch_fill(const mllm_grpo_embedding_args* a, const uint8_t* busy, int64_t from, bool beside, cudaStream_t s) {
-  const int64_t rows_per = kMostWords / (a->hidden * elem(a->out_dtype) / int64_t(sizeof(W)));
-  for (int64_t r0 = from; r0 < a->vocab; r0 += rows_per) {
-    const FillParams f = fill_params<W>(a, busy, r0, a->vocab - r0 < rows_per ? a->vocab - r0 : rows_per);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(fill_ctas(f));
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = beside && r0 == from ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, fill_kernel<W>, f);
-    count_launch();
+static int64_t rows_per_fill(const mllm_grpo_embedding_args* a) { return kMostWords / (a->hidden * elem(a->out_dtype) / int64_t(sizeof(W))); }
+
+template <typename W>
+static cudaError_t launch_fill(const mllm_grpo_embedding_args* a, const uint8_t* busy, int64_t from, int64_t to, cudaStream_t s) {
+  const int64_t rows_per = rows_per_fill<W>(a);
+  for (int64_t r0 = from; r0 < to; r0 += rows_per) {
+    const FillParams f = fill_params<W>(a, busy, r0, to - r0 < rows_per ? to - r0 : rows_per);
+    fill_kernel<W><<<fill_ctas(f), kThreads, 0, s>>>(f);
+    const cudaError_t e = done();
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
+}
+
+// Bytes of zeros that take as long as the sort (14 us, 25 us for 32768 tokens), and somewhat more: 18 us and 36.
+static int64_t sort_bytes(int64_t n_tokens) { return (int64_t(128) << 20) + n_tokens * 4096; }
+
+// Beside the sort: the zeros of the first p.filled rows, the list and the sums of runs.
+template <typename T, int EV, typename W>
+static cudaError_t launch_fill_runs(const mllm_grpo_embedding_args* a, const GradParams& p, uint32_t row_vecs, cudaStream_t s) {
+  const int64_t rows_per = rows_per_fill<W>(a), rows = p.filled < rows_per ? p.filled : rows_per;
+  const FillParams f = fill_params<W>(a, nullptr, 0, rows);
+  const uint32_t warps = kThreads / 32, runs = (p.n + kRun - 1) / kRun, fills = fill_ctas(f);
+  Beside b;
+  b.row_vecs = row_vecs;
+  b.parts = (row_vecs + 31) / 32;
+  b.list_ctas = (runs + warps - 1) / warps;
+  b.sum_ctas = uint32_t((int64_t(runs) * b.parts + warps - 1) / warps);
+  // late enough for the sort to be done
+  const int64_t late = sort_bytes(p.n) / (kThreads * kVecs * int64_t(sizeof(W)));
+  b.first = uint32_t(fills < late ? fills : late);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(fills + b.list_ctas + b.sum_ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fill_runs_kernel<T, EV, W>, p, f, b);
+  count_launch();
+  return e == cudaSuccess ? launch_fill<W>(a, nullptr, rows, p.filled, s) : e;
 }
 
 template <typename T, typename O, int EV, typename W>
@@ -683,16 +732,15 @@ static cudaError_t launch_rows_w(const mllm_grpo_embedding_args* a, GradParams p
   // four CTAs are resident per SM: with many rows they are all busy with rows at first
   const int64_t most = 148 * 4, items = (int64_t(p.n) * p.group + kThreads - 1) / kThreads;
   p.row_ctas = uint32_t(items < most ? items : most);
-  if (a->accumulate || p.filled) {
+  if (p.filled == p.vocab) {
     grad_rows_kernel<T, O, EV, W><<<p.row_ctas, kThreads, 0, s>>>(p, FillParams{0, 0, 1, FastDiv(1), nullptr, nullptr});
     return done();
   }
-  const int64_t rows_per = kMostWords / (a->hidden * elem(a->out_dtype) / int64_t(sizeof(W)));
-  const int64_t rows = a->vocab < rows_per ? a->vocab : rows_per;
-  const FillParams f = fill_params<W>(a, p.busy, 0, rows);
+  const int64_t left = a->vocab - p.filled, rows = left < rows_per_fill<W>(a) ? left : rows_per_fill<W>(a);
+  const FillParams f = fill_params<W>(a, p.busy, p.filled, rows);
   grad_rows_kernel<T, O, EV, W><<<p.row_ctas + fill_ctas(f), kThreads, 0, s>>>(p, f);
   const cudaError_t e = done();
-  return e == cudaSuccess ? launch_fill<W>(a, p.busy, rows, false, s) : e;
+  return e == cudaSuccess ? launch_fill<W>(a, p.busy, p.filled + rows, p.vocab, s) : e;
 }
 
 // Zeros are written in the widest words that every row allows: 16 bytes, or an element.
@@ -702,19 +750,40 @@ static bool wide_rows(const mllm_grpo_embedding_args* a) {
 }
 
 // The whole gradient's zeros.
-static cudaError_t launch_zeros(const mllm_grpo_embedding_args* a, bool beside, cudaStream_t s) {
-  if (wide_rows(a)) return launch_fill<uint4>(a, nullptr, 0, beside, s);
-  return a->out_dtype == MLLM_GRPO_F32 ? launch_fill<uint32_t>(a, nullptr, 0, beside, s)
-                                       : launch_fill<uint16_t>(a, nullptr, 0, beside, s);
+static cudaError_t launch_zeros(const mllm_grpo_embedding_args* a, cudaStream_t s) {
+  if (wide_rows(a)) return launch_fill<uint4>(a, nullptr, 0, a->vocab, s);
+  return a->out_dtype == MLLM_GRPO_F32 ? launch_fill<uint32_t>(a, nullptr, 0, a->vocab, s) : launch_fill<uint16_t>(a, nullptr, 0, a->vocab, s);
 }
 
-// Whether the zeros of the whole gradient are written beside the sort, and the rows that have tokens after that: these
-// are then written twice, which costs less than the sort where they are few or narrow.  151936 f32 rows, this way / with
-// the zeros in the last launch: 2048 tokens of width 896 84 / 94 us, 32768 of them 127 / 135, 4096 of width 3584
-// 322 / 328; but 8192 of width 3584 346 / 335, 16384 of them 390 / 366.
-static bool rows_after_fill(const mllm_grpo_embedding_args* a) {
+// Rows whose zeros are written beside the sort.  Those of them that have tokens are written twice.  All rows where that
+// costs little, because few or narrow rows can have tokens: 151936 f32 rows, this way / all zeros in the last launch,
+// 2048 tokens of width 896 81 / 94 us, 32768 of them 124 / 135, 4096 of width 3584 317 / 328.  (But 16384 of width 3584
+// 390 / 366.)  Otherwise as many as fill the time until the rows with tokens are known: 8192 of width 3584 322, 16384
+// 352 (three times as many: 357, six times: 364).
+static int64_t rows_beside(const mllm_grpo_embedding_args* a) {
   const int64_t row = a->hidden * elem(a->out_dtype);
-  return !a->accumulate && (row <= 4096 || a->n_tokens * row <= int64_t(64) << 20);
+  if (a->accumulate || row <= 4096 || a->n_tokens * row <= int64_t(64) << 20) return a->vocab;
+  const int64_t rows = sort_bytes(a->n_tokens) / row + 1;
+  return rows < a->vocab ? rows : a->vocab;
+}
+
+template <typename T, int EV>
+static cudaError_t launch_runs(const mllm_grpo_embedding_args* a, const GradParams& p, cudaStream_t s) {
+  const auto go = [&](auto wide, uint32_t row_vecs) {
+    constexpr int V = decltype(wide)::value;
+    if (!p.accumulate) {
+      if (wide_rows(a)) return launch_fill_runs<T, V, uint4>(a, p, row_vecs, s);
+      return a->out_dtype == MLLM_GRPO_F32 ? launch_fill_runs<T, V, uint32_t>(a, p, row_vecs, s)
+                                           : launch_fill_runs<T, V, uint16_t>(a, p, row_vecs, s);
+    }
+    const uint32_t runs = (p.n + kRun - 1) / kRun, threads = row_vecs <= 32 ? 32 : (row_vecs <= 64 ? 64 : 128);
+    run_kernel<T, V><<<dim3(runs, (row_vecs + threads - 1) / threads + 1), threads, 0, s>>>(p, row_vecs);
+    return done();
+  };
+  constexpr int kWide = 16 / int(sizeof(T));
+  if (vec_of(p.hidden, kWide, p.grad, p.grad_stride, sizeof(T), p.run, p.hidden, 2) == kWide)
+    return go(std::integral_constant<int, kWide>(), p.hidden / kWide);
+  return go(std::integral_constant<int, EV>(), p.row_vecs);
 }
 
 template <typename T, typename O, int EV>
@@ -725,7 +794,7 @@ static cudaError_t launch_rows(const mllm_grpo_embedding_args* a, const GradPara
 
 template <typename T, int EV>
 static cudaError_t launch_grad_ev(const mllm_grpo_embedding_args* a, const GradParams& p, cudaStream_t s) {
-  const cudaError_t e = launch_runs<T, EV>(p, s);
+  const cudaError_t e = launch_runs<T, EV>(a, p, s);
   if (e != cudaSuccess) return e;
   if (a->out_dtype == MLLM_GRPO_F32) return launch_rows<T, float, EV>(a, p, s);
   if (a->out_dtype == MLLM_GRPO_F16) return launch_rows<T, __half, EV>(a, p, s);
@@ -870,12 +939,11 @@ int mllm_grpo_embedding_grad(const mllm_grpo_embedding_args* a, void* stream) {
   const int last = (q.passes - 1) & 1;
   cudaError_t e = cudaSuccess;
   if (n) {
-    const bool filled = emb::rows_after_fill(a);
-    e = emb::launch_sort(q, !a->accumulate && !filled, s);
-    if (e == cudaSuccess && filled) e = emb::launch_zeros(a, true, s);
+    const int64_t filled = emb::rows_beside(a);
+    e = emb::launch_sort(q, filled < a->vocab, s);
     if (e != cudaSuccess) return record_cuda_error(e);
     emb::GradParams p{a->token_stride, a->weight_stride, n, uint32_t(a->hidden), uint32_t(a->vocab), 0, a->accumulate ? 1u : 0u,
-                      filled ? 1u : 0u, 0, 0, 0, emb::FastDiv(1), a->scale, q.key[last], q.idx[last], reinterpret_cast<uint8_t*>(q.busy), lists,
+                      uint32_t(filled), 0, 0, 0, emb::FastDiv(1), a->scale, q.key[last], q.idx[last], reinterpret_cast<uint8_t*>(q.busy), lists,
                       a->grad_out, a->dweight,
                       reinterpret_cast<float*>(w + list + 16 + int64_t(n) * int64_t(sizeof(emb::Light)))};
     if (a->dtype == MLLM_GRPO_BF16)
@@ -885,7 +953,7 @@ int mllm_grpo_embedding_grad(const mllm_grpo_embedding_args* a, void* stream) {
     else
       e = emb::launch_grad_t<float>(a, p, s);
   }
-  if (n == 0) e = emb::launch_zeros(a, false, s);  // the accumulated form has returned
+  if (n == 0) e = emb::launch_zeros(a, s);  // the accumulated form has returned
   return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);
 }
 

@@ -235,3 +235,30 @@ def test_captured_backward(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(grad, want[k])
+
+
+@pytest.mark.parametrize("H,out_dtype", [(2048, torch.float32), (2047, torch.float32), (4096, torch.bfloat16)])
+def test_grad_of_many_wide_rows(cuda, H, out_dtype):
+    """So many wide rows may have tokens that only the first ones get their zeros beside the sort."""
+    V, N = 30000, 9001
+    gen = torch.Generator().manual_seed(14)
+    ids = torch.randint(0, V, (N,), generator=gen)
+    ids[100:300], ids[4000:4020], ids[-1], ids[0] = 29990, 20000, V - 1, 0
+    ids = ids.to(cuda)
+    x = _rows(N, H, torch.bfloat16, 14, cuda)
+    poison = torch.full((V, H), float("nan"), dtype=out_dtype, device=cuda)  # the next allocation of this size
+    del poison
+    out = G.embedding_grad(x, ids, V, scale=0.5, dtype=out_dtype)
+    ref, mag, n = _grad_ref(x, ids, V, 0.5)
+    R.assert_within(out, ref, _grad_bound(ref, mag, n, out_dtype), "dweight")
+
+
+def test_grad_beyond_2_to_31_words(cuda):
+    """16-bit rows at odd addresses are filled an element at a time, in several launches."""
+    V, H = 70001, 32769
+    ids = torch.tensor([0, 65535, V - 1, 65533, 65534], device=cuda)
+    x = _rows(5, H, torch.bfloat16, 15, cuda)
+    out = G.embedding_grad(x, ids, V, dtype=torch.bfloat16)
+    assert torch.equal(out[ids], x)
+    out[ids] = 0
+    assert not any(part.any() for part in out.split(4096))
