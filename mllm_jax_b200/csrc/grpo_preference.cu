@@ -337,6 +337,7 @@ __global__ void __launch_bounds__(THREADS) pref_pairs_kernel(const Params p) {
   __shared__ SeqSums sums[2 * kHalfWarps];
   __shared__ float2 k_shared;
   __shared__ bool last;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int side = threadIdx.x / kHalf, tid = threadIdx.x % kHalf;
   const int64_t pair = blockIdx.x, s = side * p.n_pairs + pair;
   const SeqSums mine = warp_add(sequence_sums<LOGPS>(p, s, tid, kHalf));
@@ -387,16 +388,17 @@ __global__ void __launch_bounds__(THREADS) pref_dlogits_kernel(const Params p) {
   uint16_t* d16 = p.dlogits + r * p.row_stride + c0;
   float g = 0.f, lse = 0.f;
   int64_t cl = -1;
-  if (t < p.scored_rows) {
-    float m;
-    if (live_token(p, b, t, &m)) {
-      const float gs = p.grad_scale_dev ? *p.grad_scale_dev : p.grad_scale;
-      g = -p.coef[b] * m * gs;
-      lse = p.lse[b * p.scored_rows + t];
-      int64_t c = p.ids[b * p.ids_stride + t];
-      c = c < 0 ? 0 : (c >= p.vocab ? p.vocab - 1 : c);
-      cl = c - c0;
-    }
+  float m = 0.f;
+  const bool live = t < p.scored_rows && live_token(p, b, t, &m);
+  // beside pref_pairs_kernel: zeros need nothing of it; some CTA has to end after it in any case
+  if (live || blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (live) {
+    const float gs = p.grad_scale_dev ? *p.grad_scale_dev : p.grad_scale;
+    g = -p.coef[b] * m * gs;
+    lse = p.lse[b * p.scored_rows + t];
+    int64_t c = p.ids[b * p.ids_stride + t];
+    c = c < 0 ? 0 : (c >= p.vocab ? p.vocab - 1 : c);
+    cl = c - c0;
   }
   const SoftCap sc(CAP ? p.softcap : 1.0f);
   if (!SCALAR) {
@@ -449,24 +451,35 @@ static cudaError_t launch_forward(const Params& p, cudaStream_t s) {
   return launch_pairs<false>(p, s);
 }
 
-template <bool CAP>
-static void launch_backward_t(const Params& p, unsigned grid, bool same_phase, cudaStream_t s) {
-  if (!same_phase)
-    pref_dlogits_kernel<256, 4, CAP, true><<<grid, 256, 0, s>>>(p);
-  else if (p.split_cols <= 16384)
-    pref_dlogits_kernel<128, 4, CAP, false><<<grid, 128, 0, s>>>(p);
-  else
-    pref_dlogits_kernel<512, 4, CAP, false><<<grid, 512, 0, s>>>(p);
+template <typename K>
+static cudaError_t launch_rows(K* kernel, const Params& p, unsigned grid, unsigned threads, bool beside, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = beside ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  count_launch();
+  return e;
 }
 
-static cudaError_t launch_backward(const Params& p, cudaStream_t s) {
+template <bool CAP>
+static cudaError_t launch_backward_t(const Params& p, unsigned grid, bool same_phase, bool beside, cudaStream_t s) {
+  if (!same_phase) return launch_rows(pref_dlogits_kernel<256, 4, CAP, true>, p, grid, 256, beside, s);
+  if (p.split_cols <= 16384) return launch_rows(pref_dlogits_kernel<128, 4, CAP, false>, p, grid, 128, beside, s);
+  return launch_rows(pref_dlogits_kernel<512, 4, CAP, false>, p, grid, 512, beside, s);
+}
+
+// beside: right behind launch_forward, whose last launch it need not wait for as a whole.
+static cudaError_t launch_backward(const Params& p, bool beside, cudaStream_t s) {
   const unsigned grid = unsigned(2 * p.n_pairs * p.seq_rows * p.splits);
   const bool same_phase = ((reinterpret_cast<uintptr_t>(p.logits) ^ reinterpret_cast<uintptr_t>(p.dlogits)) & 15) == 0;
-  if (p.softcap > 0.f)
-    launch_backward_t<true>(p, grid, same_phase, s);
-  else
-    launch_backward_t<false>(p, grid, same_phase, s);
-  return done();
+  return p.softcap > 0.f ? launch_backward_t<true>(p, grid, same_phase, beside, s)
+                         : launch_backward_t<false>(p, grid, same_phase, beside, s);
 }
 
 static bool aligned(const void* q, size_t a) { return (reinterpret_cast<uintptr_t>(q) & (a - 1)) == 0; }
@@ -583,7 +596,7 @@ int mllm_grpo_preference_bwd(const mllm_grpo_preference_args* args, void* stream
   pref::Params p;
   const int st = pref::bind(args, pref::kLogits | pref::kBackward, &p);
   if (st) return st;
-  const cudaError_t e = pref::launch_backward(p, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = pref::launch_backward(p, false, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);
 }
 
@@ -592,7 +605,7 @@ int mllm_grpo_preference_fwd_bwd(const mllm_grpo_preference_args* args, void* st
   const int st = pref::bind(args, pref::kLogits | pref::kForward | pref::kBackward, &p);
   if (st) return st;
   cudaError_t e = pref::launch_forward(p, static_cast<cudaStream_t>(stream));
-  if (e == cudaSuccess) e = pref::launch_backward(p, static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess) e = pref::launch_backward(p, true, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);
 }
 
