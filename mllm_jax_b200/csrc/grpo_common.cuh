@@ -312,4 +312,19 @@ __device__ __forceinline__ TokenOut token_epilogue(const KernelParams& p, int64_
   return token_epilogue_core<ENT>(p, st, yc, load_token_side(p, n, b));
 }
 
+// n / d for n < 2^32 by a multiplication (d > 0): the quotient of Granlund and Montgomery's method.
+struct FastDiv {
+  uint32_t d, m, s;
+  explicit FastDiv(uint32_t div) : d(div) {
+    uint32_t l = 0;
+    while (l < 32 && (uint64_t(1) << l) < div) ++l;
+    m = uint32_t((((uint64_t(1) << l) - div) << 32) / div + 1);
+    s = l;
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    const uint32_t t = __umulhi(m, n);
+    return s == 0 ? n : (t + ((n - t) >> 1)) >> (s - 1);
+  }
+};
+
 }  // namespace grpo

@@ -33,21 +33,6 @@ namespace emb {
 
 constexpr int kThreads = 256;
 
-// n / d for n < 2^32 by a multiplication (d > 0): the quotient of Granlund and Montgomery's method.
-struct FastDiv {
-  uint32_t d, m, s;
-  explicit FastDiv(uint32_t div) : d(div) {
-    uint32_t l = 0;
-    while (l < 32 && (uint64_t(1) << l) < div) ++l;
-    m = uint32_t((((uint64_t(1) << l) - div) << 32) / div + 1);
-    s = l;
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const {
-    const uint32_t t = __umulhi(m, n);
-    return s == 0 ? n : (t + ((n - t) >> 1)) >> (s - 1);
-  }
-};
-
 template <typename T>
 struct Conv;
 template <>
@@ -300,10 +285,13 @@ struct FillParams {
   FastDiv by_row;
   const uint8_t* busy;  // of this launch's rows; null: no row has tokens
   void* out;
+  uint16_t* end;  // 2-byte pieces behind the last whole word (fewer than 8)
+  uint32_t pieces;
 };
 template <typename W>
 __device__ __forceinline__ void fill(const FillParams& p, uint32_t block) {
   const uint32_t base = block * uint32_t(kThreads * kVecs) + threadIdx.x;
+  if (block == 0 && threadIdx.x < p.pieces) p.end[threadIdx.x] = 0;
   uint32_t skip = 0;
   if (p.busy) {
 #pragma unroll
@@ -675,11 +663,21 @@ template <typename W>
 static FillParams fill_params(const mllm_grpo_embedding_args* a, const uint8_t* busy, int64_t r0, int64_t rows) {
   const int64_t eo = elem(a->out_dtype), row_words = a->hidden * eo / int64_t(sizeof(W));
   FillParams f{a->weight_stride * eo / int64_t(sizeof(W)), uint32_t(rows * row_words), uint32_t(row_words),
-               FastDiv(uint32_t(row_words)), busy ? busy + r0 : nullptr, nullptr};
+               FastDiv(uint32_t(row_words)), busy ? busy + r0 : nullptr, nullptr, nullptr, 0};
   f.out = static_cast<W*>(a->dweight) + r0 * f.stride;
   return f;
 }
-static unsigned fill_ctas(const FillParams& f) { return (f.total + kThreads * kVecs - 1) / (kThreads * kVecs); }
+// A whole table whose rows follow one another, as one row of 16-byte words, whatever its width (odd widths an element at
+// a time: 3.3 TB/s).
+static bool flat_table(const mllm_grpo_embedding_args* a) {
+  return a->weight_stride == a->hidden && aligned(a->dweight, 16) && a->vocab * a->hidden * elem(a->out_dtype) / 16 <= kMostWords;
+}
+static FillParams flat_params(const mllm_grpo_embedding_args* a) {
+  const int64_t bytes = a->vocab * a->hidden * elem(a->out_dtype), words = bytes / 16;
+  return FillParams{0, uint32_t(words), uint32_t(words), FastDiv(words ? uint32_t(words) : 1u), nullptr, a->dweight,
+                    reinterpret_cast<uint16_t*>(static_cast<char*>(a->dweight) + words * 16), uint32_t(bytes % 16 / 2)};
+}
+static unsigned fill_ctas(const FillParams& f) { return f.total / (kThreads * kVecs) + 1; }
 
 template <typename W>
 static int64_t rows_per_fill(const mllm_grpo_embedding_args* a) { return kMostWords / (a->hidden * elem(a->out_dtype) / int64_t(sizeof(W))); }
@@ -702,8 +700,9 @@ static int64_t sort_bytes(int64_t n_tokens) { return (int64_t(128) << 20) + n_to
 // Beside the sort: the zeros of the first p.filled rows, the list and the sums of runs.
 template <typename T, int EV, typename W>
 static cudaError_t launch_fill_runs(const mllm_grpo_embedding_args* a, const GradParams& p, uint32_t row_vecs, cudaStream_t s) {
-  const int64_t rows_per = rows_per_fill<W>(a), rows = p.filled < rows_per ? p.filled : rows_per;
-  const FillParams f = fill_params<W>(a, nullptr, 0, rows);
+  const bool flat = sizeof(W) == 16 && p.filled == p.vocab && flat_table(a);
+  const int64_t rows_per = flat ? p.vocab : rows_per_fill<W>(a), rows = p.filled < rows_per ? p.filled : rows_per;
+  const FillParams f = flat ? flat_params(a) : fill_params<W>(a, nullptr, 0, rows);
   const uint32_t warps = kThreads / 32, runs = (p.n + kRun - 1) / kRun, fills = fill_ctas(f);
   Beside b;
   b.row_vecs = row_vecs;
@@ -724,7 +723,7 @@ static cudaError_t launch_fill_runs(const mllm_grpo_embedding_args* a, const Gra
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, fill_runs_kernel<T, EV, W>, p, f, b);
   count_launch();
-  return e == cudaSuccess ? launch_fill<W>(a, nullptr, rows, p.filled, s) : e;
+  return e == cudaSuccess && rows < p.filled ? launch_fill<W>(a, nullptr, rows, p.filled, s) : e;
 }
 
 template <typename T, typename O, int EV, typename W>
@@ -733,7 +732,7 @@ static cudaError_t launch_rows_w(const mllm_grpo_embedding_args* a, GradParams p
   const int64_t most = 148 * 4, items = (int64_t(p.n) * p.group + kThreads - 1) / kThreads;
   p.row_ctas = uint32_t(items < most ? items : most);
   if (p.filled == p.vocab) {
-    grad_rows_kernel<T, O, EV, W><<<p.row_ctas, kThreads, 0, s>>>(p, FillParams{0, 0, 1, FastDiv(1), nullptr, nullptr});
+    grad_rows_kernel<T, O, EV, W><<<p.row_ctas, kThreads, 0, s>>>(p, FillParams{0, 0, 1, FastDiv(1), nullptr, nullptr, nullptr, 0});
     return done();
   }
   const int64_t left = a->vocab - p.filled, rows = left < rows_per_fill<W>(a) ? left : rows_per_fill<W>(a);
@@ -751,6 +750,11 @@ static bool wide_rows(const mllm_grpo_embedding_args* a) {
 
 // The whole gradient's zeros.
 static cudaError_t launch_zeros(const mllm_grpo_embedding_args* a, cudaStream_t s) {
+  if (flat_table(a)) {
+    const FillParams f = flat_params(a);
+    fill_kernel<uint4><<<fill_ctas(f), kThreads, 0, s>>>(f);
+    return done();
+  }
   if (wide_rows(a)) return launch_fill<uint4>(a, nullptr, 0, a->vocab, s);
   return a->out_dtype == MLLM_GRPO_F32 ? launch_fill<uint32_t>(a, nullptr, 0, a->vocab, s) : launch_fill<uint16_t>(a, nullptr, 0, a->vocab, s);
 }
@@ -772,7 +776,7 @@ static cudaError_t launch_runs(const mllm_grpo_embedding_args* a, const GradPara
   const auto go = [&](auto wide, uint32_t row_vecs) {
     constexpr int V = decltype(wide)::value;
     if (!p.accumulate) {
-      if (wide_rows(a)) return launch_fill_runs<T, V, uint4>(a, p, row_vecs, s);
+      if (wide_rows(a) || (p.filled == p.vocab && flat_table(a))) return launch_fill_runs<T, V, uint4>(a, p, row_vecs, s);
       return a->out_dtype == MLLM_GRPO_F32 ? launch_fill_runs<T, V, uint32_t>(a, p, row_vecs, s)
                                            : launch_fill_runs<T, V, uint16_t>(a, p, row_vecs, s);
     }
@@ -878,7 +882,7 @@ int mllm_grpo_embedding_lookup(const mllm_grpo_embedding_args* a, void* stream) 
   const int64_t es = emb::elem(a->dtype);
   if (!emb::aligned(a->weight, es) || !emb::aligned(a->out, es)) return MLLM_GRPO_ERR_ALIGNMENT;
   emb::LookupParams p{a->weight_stride, a->token_stride, a->vocab_start, a->vocab,
-                      a->vocab_total ? a->vocab_total : a->vocab_start + a->vocab, 0, 0, emb::FastDiv(1), a->scale,
+                      a->vocab_total ? a->vocab_total : a->vocab_start + a->vocab, 0, 0, FastDiv(1), a->scale,
                       a->ids, a->weight, a->out, a->device_status};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
@@ -943,7 +947,7 @@ int mllm_grpo_embedding_grad(const mllm_grpo_embedding_args* a, void* stream) {
     e = emb::launch_sort(q, filled < a->vocab, s);
     if (e != cudaSuccess) return record_cuda_error(e);
     emb::GradParams p{a->token_stride, a->weight_stride, n, uint32_t(a->hidden), uint32_t(a->vocab), 0, a->accumulate ? 1u : 0u,
-                      uint32_t(filled), 0, 0, 0, emb::FastDiv(1), a->scale, q.key[last], q.idx[last], reinterpret_cast<uint8_t*>(q.busy), lists,
+                      uint32_t(filled), 0, 0, 0, FastDiv(1), a->scale, q.key[last], q.idx[last], reinterpret_cast<uint8_t*>(q.busy), lists,
                       a->grad_out, a->dweight,
                       reinterpret_cast<float*>(w + list + 16 + int64_t(n) * int64_t(sizeof(emb::Light)))};
     if (a->dtype == MLLM_GRPO_BF16)

@@ -34,6 +34,7 @@ struct IsBf16<__nv_bfloat16> {
 
 struct Params {
   int64_t rows, cols, x_stride, q_stride, blocks;  // blocks along a row
+  FastDiv by_row;
   const void* x;
   uint8_t* q;
   float* scales;
@@ -128,10 +129,10 @@ struct Word<1> {
   using type = uint8_t;
 };
 
-// y rounded to 19 bits: (33 y) - (33 y - y) keeps the upper part.
-__device__ __forceinline__ float snap(float y) {
-  const float c = __fmul_rn(y, 33.0f);
-  return __fsub_rn(c, __fsub_rn(c, y));
+// Two elements times r, rounded to 19 bits: with y = x r, (33 y) - (33 y - y) keeps the upper part.
+__device__ __forceinline__ void scaled(float& a, float& b, float r) {
+  const f32x2 y = mul2(pack2(a, b), pack2(r, r)), c = mul2(y, pack2(33.0f, 33.0f)), minus = pack2(-1.0f, -1.0f);
+  unpack2(fma2(fma2(y, minus, c), minus, c), a, b);
 }
 
 // Two f32 -> two e4m3 bytes (first in the low byte), to nearest even; a NaN becomes the e4m3 NaN.
@@ -148,7 +149,10 @@ __device__ __forceinline__ float factor(float amax, float* scale) {
   return __fdiv_rn(kMost, top);
 }
 
-__device__ __forceinline__ uint32_t pair(float a, float b, float r) { return to_e4m3x2(snap(a * r), snap(b * r)); }
+__device__ __forceinline__ uint32_t pair(float a, float b, float r) {
+  scaled(a, b, r);
+  return to_e4m3x2(a, b);
+}
 template <typename T, int EV>
 __device__ __forceinline__ typename Word<EV>::type convert(const Raw<T, EV>& x, float r) {
   if constexpr (EV == 8) {
@@ -169,38 +173,63 @@ template <typename T, int EV>
 struct RowGroup {
   static constexpr int kThreadsPerBlock = 128 / EV > 32 ? 32 : 128 / EV;
   static constexpr int kVecs = 128 / (kThreadsPerBlock * EV);
+  static constexpr int kAtOnce = 4;
 };
+// A group of threads takes four blocks, all of them on their way before the first is looked at; their maxima are found
+// together, and each of the two divisions of a scale is done by one lane for its block while others do theirs.  65536 x
+// 3584 bf16 in 121 us, 141965 x 477 in 83 (one block at a time, every lane dividing, its place from a 64-bit division:
+// 181 and 131 us).
 template <typename T, int EV>
-__global__ void __launch_bounds__(kThreads) row_blocks_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 5) row_blocks_kernel(const Params p) {
   constexpr int G = RowGroup<T, EV>::kThreadsPerBlock;
   constexpr int U = RowGroup<T, EV>::kVecs;
-  const int64_t g = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / G;  // block of the whole matrix
+  constexpr int R = RowGroup<T, EV>::kAtOnce;
+  constexpr int GROUPS = kThreads / G;
   const int l = threadIdx.x % G;
-  const int64_t row = g / p.blocks, b = g - row * p.blocks;
-  const bool in = row < p.rows;
-  const int64_t c0 = b * 128;
-  const T* x = static_cast<const T*>(p.x) + row * p.x_stride + c0;
-  Raw<T, EV> v[U];
-  AbsMax<T> top;
+  const uint32_t first = blockIdx.x * uint32_t(GROUPS * R) + threadIdx.x / G;  // block of this launch's rows
+  const uint32_t rows = uint32_t(p.rows), blocks = uint32_t(p.blocks);
+  Raw<T, EV> v[R][U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int c = (u * G + l) * EV;
-    v[u].zero();
-    if (in && c0 + c < p.cols) v[u].load(x + c);
-    top.add(v[u]);
+  for (int r = 0; r < R; ++r) {
+    const uint32_t row = p.by_row.div(first + r * GROUPS), c0 = (first + r * GROUPS - row * blocks) * 128;
+    const T* x = static_cast<const T*>(p.x) + row * p.x_stride + c0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = (u * G + l) * EV;
+      v[r][u].zero();
+      if (row < rows && c0 + c < uint32_t(p.cols)) v[r][u].load(x + c);
+    }
   }
-  float amax = top.value();
+  // maxima of all R blocks at once: the first two steps leave lane l with block l % 4
+  static_assert(R == 4, "");
+  float m[R];
 #pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  float scale;
-  const float r = factor(amax, &scale);
-  if (!in) return;
-  if (l == 0) p.scales[g] = scale;
-  uint8_t* q = p.q + row * p.q_stride + c0;
+  for (int r = 0; r < R; ++r) {
+    AbsMax<T> top;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int c = (u * G + l) * EV;
-    if (c0 + c < p.cols) *reinterpret_cast<typename Word<EV>::type*>(q + c) = convert<T, EV>(v[u], r);
+    for (int u = 0; u < U; ++u) top.add(v[r][u]);
+    m[r] = top.value();
+  }
+  const bool odd = l & 1, upper = l & 2;
+  const float m0 = fmaxf(odd ? m[1] : m[0], __shfl_xor_sync(0xffffffffu, odd ? m[0] : m[1], 1));
+  const float m1 = fmaxf(odd ? m[3] : m[2], __shfl_xor_sync(0xffffffffu, odd ? m[2] : m[3], 1));
+  float amax = fmaxf(upper ? m1 : m0, __shfl_xor_sync(0xffffffffu, upper ? m0 : m1, 2));
+#pragma unroll
+  for (int o = 4; o < G; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  float my_scale;
+  const float mine = factor(amax, &my_scale);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float f = __shfl_sync(0xffffffffu, mine, r, G), scale = __shfl_sync(0xffffffffu, my_scale, r, G);
+    const uint32_t row = p.by_row.div(first + r * GROUPS), c0 = (first + r * GROUPS - row * blocks) * 128;
+    if (row >= rows) continue;
+    if (l == 0) p.scales[first + r * GROUPS] = scale;
+    uint8_t* q = p.q + row * p.q_stride + c0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = (u * G + l) * EV;
+      if (c0 + c < uint32_t(p.cols)) *reinterpret_cast<typename Word<EV>::type*>(q + c) = convert<T, EV>(v[r][u], f);
+    }
   }
 }
 
@@ -244,12 +273,23 @@ __global__ void __launch_bounds__(kThreads, 16 * EV >= 64 && sizeof(T) == 2 ? 4 
 template <typename T, int EV>
 static cudaError_t launch(const Params& p, int block_rows, cudaStream_t s) {
   if (block_rows == 1) {
-    constexpr int G = RowGroup<T, EV>::kThreadsPerBlock;
-    const int64_t groups = p.rows * p.blocks;
-    row_blocks_kernel<T, EV><<<unsigned((groups + kThreads / G - 1) / (kThreads / G)), kThreads, 0, s>>>(p);
-  } else {
-    tile_blocks_kernel<T, EV><<<unsigned((p.rows + 127) / 128 * p.blocks), kThreads, 0, s>>>(p);
+    constexpr int64_t kPer = kThreads / RowGroup<T, EV>::kThreadsPerBlock * RowGroup<T, EV>::kAtOnce;
+    // blocks are counted in 32 bits: more than 2^31 of them go in several launches
+    const int64_t rows_per = (int64_t(1) << 31) / p.blocks;
+    for (int64_t r0 = 0; r0 < p.rows; r0 += rows_per) {
+      Params part = p;
+      part.rows = p.rows - r0 < rows_per ? p.rows - r0 : rows_per;
+      part.x = static_cast<const T*>(p.x) + r0 * p.x_stride;
+      part.q = p.q + r0 * p.q_stride;
+      part.scales = p.scales + r0 * p.blocks;
+      row_blocks_kernel<T, EV><<<unsigned((part.rows * part.blocks + kPer - 1) / kPer), kThreads, 0, s>>>(part);
+      count_launch();
+      const cudaError_t e = cudaGetLastError();
+      if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
   }
+  tile_blocks_kernel<T, EV><<<unsigned((p.rows + 127) / 128 * p.blocks), kThreads, 0, s>>>(p);
   count_launch();
   return cudaGetLastError();
 }
@@ -279,13 +319,12 @@ extern "C" int mllm_lm_head_fp8_quantize(const mllm_lm_head_fp8_quantize_args* a
     return MLLM_GRPO_ERR_BAD_ATTRIBUTE;
   const int64_t blocks = (a->cols - 1) / 128 + 1;
   if (a->rows > (int64_t(1) << 32) || blocks > (int64_t(1) << 24)) return MLLM_GRPO_ERR_TOO_LARGE;
-  // one CTA holds at least 8 row blocks, or one tile
-  if ((a->block_rows == 1 ? a->rows / 8 + 1 : a->rows / 128 + 1) * blocks > (int64_t(1) << 31) - 1) return MLLM_GRPO_ERR_TOO_LARGE;
+  if (a->block_rows != 1 && (a->rows / 128 + 1) * blocks > (int64_t(1) << 31) - 1) return MLLM_GRPO_ERR_TOO_LARGE;
   if (a->rows == 0) return MLLM_GRPO_OK;
   if (!a->x || !a->q || !a->scales) return MLLM_GRPO_ERR_NULL_POINTER;
   const uintptr_t es = a->dtype == MLLM_GRPO_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(a->x) % es || reinterpret_cast<uintptr_t>(a->scales) % 4) return MLLM_GRPO_ERR_ALIGNMENT;
-  const fp8q::Params p{a->rows, a->cols, a->x_stride, a->q_stride, blocks, a->x, static_cast<uint8_t*>(a->q), a->scales};
+  const fp8q::Params p{a->rows, a->cols, a->x_stride, a->q_stride, blocks, FastDiv(uint32_t(blocks)), a->x, static_cast<uint8_t*>(a->q), a->scales};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (a->dtype == MLLM_GRPO_BF16)

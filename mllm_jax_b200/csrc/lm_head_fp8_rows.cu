@@ -134,8 +134,12 @@ cudaError_t launch_rows(const Params& p, cudaStream_t s) {
 
 template <bool WIDE, typename O>
 cudaError_t launch_w(const Params& p, cudaStream_t s) {
-  // K over four warps; over eight where that leaves less than two CTAs per SM
-  if (p.vocab <= int64_t(2) * 148 * 32) return launch_rows<8, WIDE, O>(p, s);
+  // K over four warps; over eight where that leaves less than a CTA per SM (4096 x 4096: 4.4 us, 5.7 with four); over one
+  // or two where a warp of four would have few blocks and there are CTAs enough (142803 x 288: 11.8 us, 16.7 with four;
+  // 151936 x 1536: 43 with two, 47 with four)
+  if (p.vocab <= int64_t(148) * 32) return launch_rows<8, WIDE, O>(p, s);
+  if (p.vocab > int64_t(2) * 148 * 128 && p.k_blocks <= 8) return launch_rows<1, WIDE, O>(p, s);
+  if (p.vocab > int64_t(2) * 148 * 128 && p.k_blocks <= 14) return launch_rows<2, WIDE, O>(p, s);
   return launch_rows<4, WIDE, O>(p, s);
 }
 

@@ -254,7 +254,7 @@ def test_grad_of_many_wide_rows(cuda, H, out_dtype):
 
 
 def test_grad_beyond_2_to_31_words(cuda):
-    """16-bit rows at odd addresses are filled an element at a time, in several launches."""
+    """Rows of an odd width, more elements than 32 bits of them count."""
     V, H = 70001, 32769
     ids = torch.tensor([0, 65535, V - 1, 65533, 65534], device=cuda)
     x = _rows(5, H, torch.bfloat16, 15, cuda)
@@ -262,3 +262,28 @@ def test_grad_beyond_2_to_31_words(cuda):
     assert torch.equal(out[ids], x)
     out[ids] = 0
     assert not any(part.any() for part in out.split(4096))
+
+
+@pytest.mark.parametrize("N", [0, 40, 9000])
+@pytest.mark.parametrize("H,stride,offset", [(63, 66, 1), (64, 72, 0), (2047, 2049, 3), (5, 5, 1), (5, 5, 0)])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+def test_grad_into_strided_rows(cuda, N, H, stride, offset, out_dtype):
+    """The whole gradient into rows some distance apart, at any address (through the C ABI): what lies between and
+    behind them stays."""
+    from mllm_jax_b200 import _lib
+    V = 21001 if H > 2000 else 1003
+    gen = torch.Generator().manual_seed(16)
+    ids = torch.randint(0, V, (N,), generator=gen, dtype=torch.int32).to(cuda)
+    x = _rows(N, H, torch.bfloat16, 16, cuda) if N else torch.empty(0, H, dtype=torch.bfloat16, device=cuda)
+    buf = torch.full((offset + V * stride + 8,), 7.0, dtype=out_dtype, device=cuda)
+    a = _lib.EmbeddingArgs()
+    a.n_tokens, a.vocab, a.hidden, a.weight_stride, a.token_stride, a.scale = N, V, H, stride, H, 1.0
+    a.dtype, a.out_dtype = _lib.DTYPE_BF16, _lib.DTYPE_F32 if out_dtype is torch.float32 else _lib.DTYPE_BF16
+    work = torch.empty(_lib.load().mllm_grpo_embedding_workspace_bytes(N, H, V), dtype=torch.uint8, device=cuda)
+    a.ids, a.grad_out, a.workspace = ids.data_ptr(), x.data_ptr(), work.data_ptr()
+    a.dweight = buf.data_ptr() + offset * buf.element_size()
+    _lib.launch("mllm_grpo_embedding_grad", a, x.device)
+    rows = buf[offset:offset + V * stride].view(V, stride)
+    ref, mag, n = _grad_ref(x, ids.long(), V, 1.0)
+    R.assert_within(rows[:, :H], ref, _grad_bound(ref, mag, n, out_dtype), "dweight")
+    assert bool((rows[:, H:] == 7).all()) and bool((buf[:offset] == 7).all()) and bool((buf[offset + V * stride:] == 7).all())

@@ -269,3 +269,20 @@ def test_folded_head_clamps_ids_beyond_32_bits(cuda):
     out, want = lm_head_forward(hidden, w, ids), lm_head_forward(hidden, w, near)
     assert torch.equal(out["per_token_logps"], want["per_token_logps"])
     assert int(out["problem"].device_status) == 1 and int(want["problem"].device_status) == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 40003, 16), (3, 38017, 288), (8, 40000, 1024), (2, 38000, 1296), (5, 4800, 528), (7, 4736, 400)])
+def test_few_rows_split_by_the_inner_size(cuda, M, N, K):
+    """Each way of giving K to the warps of a CTA: one, two, four and eight of them."""
+    x, w = _operands(M, N, K, 98, cuda)
+    ref, mag = R.product(x.values, x.scales, w.values, w.scales)
+    out = G.fp8_matmul(x, w, out_dtype=torch.float32)
+    R.assert_within(out, ref, R.product_bound(ref, mag, K) + ref.abs() * R.HALF_STEP[torch.float32], f"{M}x{N}x{K}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("r,c", [(40001, 129), (3001, 546), (777, 2976), (70, 1)])
+def test_quantize_rows_by_the_four(cuda, dtype, r, c):
+    """Rows whose blocks do not come in fours, odd widths, more than one wave of CTAs."""
+    x = _x(r, c, dtype, 99, cuda)
+    _check_quantized(G.quantize_fp8(x), x, (1, 128))
