@@ -286,3 +286,20 @@ def test_quantize_rows_by_the_four(cuda, dtype, r, c):
     """Rows whose blocks do not come in fours, odd widths, more than one wave of CTAs."""
     x = _x(r, c, dtype, 99, cuda)
     _check_quantized(G.quantize_fp8(x), x, (1, 128))
+
+
+@pytest.mark.parametrize("out_dtype", TYPES)
+@pytest.mark.parametrize("M,N", [(33, 300), (300, 515), (260, 33000)])
+@pytest.mark.parametrize("shift", range(8))
+def test_product_at_every_address(cuda, out_dtype, M, N, shift):
+    """Rows of out that start at every place between 16-byte boundaries, with values behind them that stay."""
+    if M * N > 10 ** 6 and shift not in (0, 1, 6):
+        return
+    x, w = _operands(M, N, 144, 101, cuda)
+    want = G.fp8_matmul(x, w, out_dtype=out_dtype)
+    for stride in (N + shift, N + 8 + (shift & 3)):
+        buf = torch.full((shift + M * stride + 16,), 3.0, dtype=out_dtype, device=cuda)
+        out = buf[shift:shift + M * stride].view(M, stride)
+        G.fp8_matmul(x, w, out=out[:, :N])
+        assert torch.equal(out[:, :N], want)
+        assert bool((out[:, N:] == 3).all()) and bool((buf[:shift] == 3).all()) and bool((buf[shift + M * stride:] == 3).all())
