@@ -465,7 +465,8 @@ typedef struct mllm_lm_head_fp8_args {
   float* per_token_logps;     /* partials: [M] or NULL, for an unsharded head: (chosen logit - lse) / temperature */
   float* token_entropy;       /* partials: [M] or NULL, at temperature 1: lse - (sum e*y) / sumexp */
   float* lse;                 /* partials: [M] or NULL */
-  int32_t* device_status;     /* optional */
+  int32_t* device_status;     /* optional: MLLM_GRPO_DEV_* bits are ORed in */
+  int32_t* call_status;       /* partials, optional: set to this call's bits */
 } mllm_lm_head_fp8_args;
 int mllm_lm_head_fp8_matmul(const mllm_lm_head_fp8_args* args, void* stream);
 /* mllm_lm_head_partials with both operands in 8 bits.  The first n_rows records of `partials` are the rows' merged

@@ -137,6 +137,7 @@ class Fp8Args(C.Structure):
         ("hidden", C.c_void_p), ("hidden_scales", C.c_void_p), ("weight", C.c_void_p), ("weight_scales", C.c_void_p),
         ("out", C.c_void_p), ("chosen_ids", C.c_void_p), ("partials", C.c_void_p), ("per_token_logps", C.c_void_p),
         ("token_entropy", C.c_void_p), ("lse", C.c_void_p), ("device_status", C.c_void_p),
+        ("call_status", C.c_void_p),
     ]
 
 

@@ -655,7 +655,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
 
 // Partials of all column ranges of a row -> one (entry 0 of the buffer) and what follows from it: 32 rows per CTA, eight
 // threads per row.
-__global__ void __launch_bounds__(256) merge_kernel(const Params p, int entries) {
+__global__ void __launch_bounds__(256) merge_kernel(const Params p, int entries, int32_t* status) {
+  if (status && blockIdx.x == 0 && threadIdx.x == 0 && *p.device_status) atomicOr(status, *p.device_status);
   float4* const partials = p.partials;
   const int64_t n_rows = p.n_rows;
   __shared__ float4 part[8][32];
@@ -879,8 +880,10 @@ int mllm_lm_head_fp8_partials(const mllm_lm_head_fp8_args* a, void* stream) {
   if (a->vocab_start < 0 || (a->vocab_total > 0 && a->vocab_start + a->vocab > a->vocab_total)) return MLLM_GRPO_ERR_BAD_SHAPE;
   if (!(a->softcap >= 0.f) || !(a->temperature >= 0.f)) return MLLM_GRPO_ERR_BAD_ATTRIBUTE;
   if (!fp8::aligned(a->partials, 16) || !fp8::aligned(a->chosen_ids, 4) || !fp8::aligned(a->per_token_logps, 4) ||
-      !fp8::aligned(a->token_entropy, 4) || !fp8::aligned(a->lse, 4))
+      !fp8::aligned(a->token_entropy, 4) || !fp8::aligned(a->lse, 4) || !fp8::aligned(a->call_status, 4))
     return MLLM_GRPO_ERR_ALIGNMENT;
+  // one word is reported into: the call's own, added to the caller's by the last launch
+  if (a->call_status) p.device_status = a->call_status;
   const float temperature = a->temperature > 0.f ? a->temperature : 1.0f;
   if (a->token_entropy && temperature != 1.0f) return MLLM_GRPO_ERR_UNSUPPORTED;
   // a shard of the vocabulary does not know a row's log-sum-exp
@@ -894,12 +897,16 @@ int mllm_lm_head_fp8_partials(const mllm_lm_head_fp8_args* a, void* stream) {
   p.vocab_start = a->vocab_start;
   p.vocab_total = a->vocab_total > 0 ? a->vocab_total : a->vocab_start + a->vocab;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->call_status) {
+    const cudaError_t e = cudaMemsetAsync(a->call_status, 0, sizeof(int32_t), s);
+    if (e != cudaSuccess) return record_cuda_error(e);
+  }
   st = fp8::ctas_for((a->n_rows + fp8::kBM - 1) / fp8::kBM) == 2 ? fp8::launch<fp8::kFoldBN, 2, true, float>(p, a, s)
                                                                   : fp8::launch<fp8::kFoldBN, 1, true, float>(p, a, s);
   if (st) return st;
   int per, splits;
   fp8::fold_plan(a->n_rows, a->vocab, &per, &splits);
-  fp8::merge_kernel<<<unsigned((a->n_rows + 31) / 32), 256, 0, s>>>(p, splits * 2);
+  fp8::merge_kernel<<<unsigned((a->n_rows + 31) / 32), 256, 0, s>>>(p, splits * 2, a->call_status ? a->device_status : nullptr);
   count_launch();
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MLLM_GRPO_OK : record_cuda_error(e);

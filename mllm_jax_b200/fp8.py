@@ -79,33 +79,32 @@ def quantize_fp8(x: torch.Tensor, *, block: Tuple[int, int] = (1, BLOCK)) -> Fp8
     return Fp8Blocks(values, scales, block)
 
 
-def _operand(t: Fp8Blocks, name: str, block) -> Fp8Blocks:
-    """The blocks as the tensor-core kernels read them: 16-byte rows at 16-byte addresses."""
+def _operand(t: Fp8Blocks, name: str, block) -> Tuple[int, int, int, int]:
+    """Rows, columns, bytes between rows and address of the values, as the tensor-core kernels read them: 16-byte rows
+    at 16-byte addresses."""
     if t.block != block:
         raise ValueError(f"{name} must have blocks of {block}, got {t.block}")
-    v = t.values
-    if v.shape[1] % 16:
-        raise ValueError(f"the inner size must be a multiple of 16, got {v.shape[1]}")
-    if v.stride(1) != 1 or (v.shape[0] > 1 and (v.stride(0) < v.shape[1] or v.stride(0) % 16)) or v.data_ptr() % 16:
+    R, C = t.values.shape
+    row, col = t.values.stride()
+    at = t.values.data_ptr()
+    if C % 16:
+        raise ValueError(f"the inner size must be a multiple of 16, got {C}")
+    if R == 1:
+        row = C
+    if col != 1 or row < C or row % 16 or at % 16:
         raise ValueError(f"{name} needs contiguous rows that start on 16-byte boundaries")
-    return t
+    return R, C, row, at
 
 
 def _bind(x: Fp8Blocks, w: Fp8Blocks) -> _lib.Fp8Args:
-    _operand(x, "x", (1, BLOCK))
-    _operand(w, "w", (BLOCK, BLOCK))
+    M, K, x_stride, x_at = _operand(x, "x", (1, BLOCK))
+    N, w_inner, w_stride, w_at = _operand(w, "w", (BLOCK, BLOCK))
     if not x.values.is_cuda:
         raise RuntimeError("the 8-bit product needs CUDA tensors: the kernels have no CPU path")
-    if x.shape[1] != w.shape[1] or x.device != w.device or w.shape[0] < 1:
+    if K != w_inner or x.device != w.device or N < 1:
         raise ValueError(f"x {tuple(x.shape)} on {x.device} and w {tuple(w.shape)} on {w.device} do not match")
-    a = _lib.Fp8Args()
-    a.n_rows, a.vocab, a.hidden_dim = x.shape[0], w.shape[0], x.shape[1]
-    K = x.shape[1]
-    a.hidden_stride = x.values.stride(0) if x.shape[0] > 1 else K
-    a.weight_stride = w.values.stride(0) if w.shape[0] > 1 else K
-    a.hidden, a.hidden_scales = x.values.data_ptr(), x.scales.data_ptr()
-    a.weight, a.weight_scales = w.values.data_ptr(), w.scales.data_ptr()
-    return a
+    return _lib.Fp8Args(n_rows=M, vocab=N, hidden_dim=K, hidden_stride=x_stride, weight_stride=w_stride, hidden=x_at,
+                        hidden_scales=x.scales.data_ptr(), weight=w_at, weight_scales=w.scales.data_ptr())
 
 
 def fp8_matmul(x: Union[Fp8Blocks, torch.Tensor], w: Fp8Blocks, *, out_dtype: torch.dtype = torch.bfloat16,

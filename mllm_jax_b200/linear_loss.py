@@ -152,10 +152,10 @@ def _fp8_logprobs(a, hq: Fp8Blocks, weight: Fp8Blocks, token_ids, cfg: LossConfi
     if token_ids.dtype is torch.int64:
         token_ids = token_ids.clamp(-1, 2 ** 31 - 1)  # an id beyond 32 bits must not wrap to a valid one
     ids = token_ids.to(device=dev, dtype=torch.int32).contiguous()
-    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    status = torch.empty(1, dtype=torch.int32, device=dev)
     out = torch.empty(3, B, T, dtype=torch.float32, device=dev)
     lp, ent, lse = out.unbind(0)
-    a.chosen_ids, a.partials, a.device_status = ids.data_ptr(), workspace.data_ptr(), status.data_ptr()
+    a.chosen_ids, a.partials, a.call_status = ids.data_ptr(), workspace.data_ptr(), status.data_ptr()
     a.softcap, a.temperature = float(cfg.softcap) if cfg.softcap else 0.0, cfg.temperature
     a.per_token_logps, a.lse = lp.data_ptr(), lse.data_ptr()
     if cfg.compute_entropy:

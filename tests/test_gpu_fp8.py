@@ -303,3 +303,20 @@ def test_product_at_every_address(cuda, out_dtype, M, N, shift):
         G.fp8_matmul(x, w, out=out[:, :N])
         assert torch.equal(out[:, :N], want)
         assert bool((out[:, N:] == 3).all()) and bool((buf[:shift] == 3).all()) and bool((buf[shift + M * stride:] == 3).all())
+
+
+def test_call_status_beside_a_running_one(cuda):
+    """The call's own bits are set, not added up, and the caller's running word collects them (through the C ABI)."""
+    from mllm_jax_b200 import _lib
+    from mllm_jax_b200.fp8 import _bind
+    N, V, H = 5, 200, 32
+    x, w = _operands(N, V, H, 102, cuda)
+    buf = torch.empty(_lib.load().mllm_lm_head_fp8_partials_bytes(N, V), dtype=torch.uint8, device=cuda)
+    mine, running = torch.full((1,), 77, dtype=torch.int32, device=cuda), torch.full((1,), 4, dtype=torch.int32, device=cuda)
+    a = _bind(x, w)
+    a.partials, a.call_status, a.device_status = buf.data_ptr(), mine.data_ptr(), running.data_ptr()
+    for ids, bits, total in (([0, 1, 2, 3, 4], 0, 4), ([0, 1, 2, 3, V], 1, 5), ([0, 1, 2, 3, 4], 0, 5)):
+        chosen = torch.tensor(ids, dtype=torch.int32, device=cuda)
+        a.chosen_ids = chosen.data_ptr()
+        _lib.launch("mllm_lm_head_fp8_partials", a, x.device)
+        assert int(mine) == bits and int(running) == total
