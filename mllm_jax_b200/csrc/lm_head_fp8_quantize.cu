@@ -124,10 +124,6 @@ template <>
 struct Word<2> {
   using type = uint16_t;
 };
-template <>
-struct Word<1> {
-  using type = uint8_t;
-};
 
 // Two elements times r, rounded to 19 bits: with y = x r, (33 y) - (33 y - y) keeps the upper part.
 __device__ __forceinline__ void scaled(float& a, float& b, float r) {
@@ -160,10 +156,8 @@ __device__ __forceinline__ typename Word<EV>::type convert(const Raw<T, EV>& x, 
                       pair(x.get(4), x.get(5), r) | (pair(x.get(6), x.get(7), r) << 16));
   } else if constexpr (EV == 4) {
     return pair(x.get(0), x.get(1), r) | (pair(x.get(2), x.get(3), r) << 16);
-  } else if constexpr (EV == 2) {
-    return uint16_t(pair(x.get(0), x.get(1), r));
   } else {
-    return uint8_t(pair(x.get(0), 0.f, r));
+    return uint16_t(pair(x.get(0), x.get(1), r));
   }
 }
 
@@ -177,7 +171,7 @@ struct RowGroup {
 };
 // A group of threads takes four blocks, all of them on their way before the first is looked at; their maxima are found
 // together, and each of the two divisions of a scale is done by one lane for its block while others do theirs.  65536 x
-// 3584 bf16 in 121 us, 141965 x 477 in 83 (one block at a time, every lane dividing, its place from a 64-bit division:
+// 3584 bf16 in 121 us, 141965 x 477 in 73 (one block at a time, every lane dividing, its place from a 64-bit division:
 // 181 and 131 us).
 template <typename T, int EV>
 __global__ void __launch_bounds__(kThreads, 5) row_blocks_kernel(const Params p) {
@@ -226,9 +220,15 @@ __global__ void __launch_bounds__(kThreads, 5) row_blocks_kernel(const Params p)
     if (l == 0) p.scales[first + r * GROUPS] = scale;
     uint8_t* q = p.q + row * p.q_stride + c0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; u += EV == 1 ? 2 : 1) {
       const int c = (u * G + l) * EV;
-      if (c0 + c < uint32_t(p.cols)) *reinterpret_cast<typename Word<EV>::type*>(q + c) = convert<T, EV>(v[r][u], f);
+      if constexpr (EV == 1) {  // two single elements are converted together
+        const uint32_t two = pair(v[r][u].get(0), v[r][u + 1].get(0), f);
+        if (c0 + c < uint32_t(p.cols)) q[c] = uint8_t(two);
+        if (c0 + c + G < uint32_t(p.cols)) q[c + G] = uint8_t(two >> 8);
+      } else {
+        if (c0 + c < uint32_t(p.cols)) *reinterpret_cast<typename Word<EV>::type*>(q + c) = convert<T, EV>(v[r][u], f);
+      }
     }
   }
 }
@@ -266,8 +266,15 @@ __global__ void __launch_bounds__(kThreads, 16 * EV >= 64 && sizeof(T) == 2 ? 4 
   if (threadIdx.x == 0) p.scales[blockIdx.x] = scale;
   uint8_t* q = p.q + r0 * p.q_stride + c0;
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (u < mine) *reinterpret_cast<typename Word<EV>::type*>(q + u * (STEP * p.q_stride)) = convert<T, EV>(v[u], r);
+  for (int u = 0; u < U; u += EV == 1 ? 2 : 1) {
+    if constexpr (EV == 1) {
+      const uint32_t two = pair(v[u].get(0), v[u + 1].get(0), r);
+      if (u < mine) q[u * (STEP * p.q_stride)] = uint8_t(two);
+      if (u + 1 < mine) q[(u + 1) * (STEP * p.q_stride)] = uint8_t(two >> 8);
+    } else {
+      if (u < mine) *reinterpret_cast<typename Word<EV>::type*>(q + u * (STEP * p.q_stride)) = convert<T, EV>(v[u], r);
+    }
+  }
 }
 
 template <typename T, int EV>
