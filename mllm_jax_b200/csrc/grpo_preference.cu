@@ -22,6 +22,7 @@ namespace pref {
 
 constexpr int kMaxSplits = 32;
 constexpr int64_t kTargetCtas = 4736;   // 32 per SM, about half of which have a masked row and leave
+constexpr int64_t kWarpCols = 2048;
 constexpr int64_t kMinSplitCols = 8192; // 16 KB of a row per CTA at least
 // Threads per pair, for answers of more than kShortTokens and for short ones (8192 pairs of single tokens: 62 us with
 // 512, 17 with 128; 8 pairs of 1024: 6.1 and 8.1; one pair of 16384: 25 and 82).
@@ -132,15 +133,20 @@ __device__ __forceinline__ void fold_one(Acc& a, uint16_t raw, const SoftCap& sc
   a.s += ex2f(fmaf(y, kLog2e, -a.mk));
 }
 
-// One CTA per (scored row, split).  Bound by reading the unmasked rows once.
-template <int THREADS, int UNROLL, bool CAP>
-__global__ void __launch_bounds__(THREADS) pref_stats_kernel(const Params p) {
+// THREADS threads per row (threadIdx.x), ROWS rows per CTA (threadIdx.y): one, or kRowsPerCta of a warp each.
+constexpr int kRowsPerCta = 8;
+
+// One CTA (warp) per (scored row, split).  Bound by reading the unmasked rows once.
+template <int THREADS, int ROWS, int UNROLL, bool CAP>
+__global__ void __launch_bounds__(THREADS * ROWS) pref_stats_kernel(const Params p) {
   constexpr int NW = THREADS / 32;
   __shared__ float red[2][NW];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (blockIdx.x == 0 && tid < 2) p.ticket[tid] = 0u;
-  const int64_t n = blockIdx.x / unsigned(p.splits);
-  const int k = int(blockIdx.x - n * p.splits);
+  if (blockIdx.x == 0 && (ROWS == 1 || threadIdx.y == 0) && tid < 2) p.ticket[tid] = 0u;
+  const unsigned item = ROWS > 1 ? blockIdx.x * ROWS + threadIdx.y : blockIdx.x;
+  if (ROWS > 1 && item >= unsigned(2 * p.n_pairs * p.scored_rows)) return;
+  const int64_t n = item / unsigned(p.splits);
+  const int k = int(item - n * p.splits);
   float mask;
   const int64_t b = n / p.scored_rows, t = n - b * p.scored_rows;
   if (!live_token(p, b, t, &mask)) return;
@@ -178,15 +184,20 @@ __global__ void __launch_bounds__(THREADS) pref_stats_kernel(const Params p) {
   }
   const float Mw = warp_max(a.mk);
   const float Sw = warp_sum(a.s * ex2f(a.mk - Mw));
-  if (lane == 0) {
-    red[0][warp] = Mw;
-    red[1][warp] = Sw;
+  if (NW > 1) {
+    if (lane == 0) {
+      red[0][warp] = Mw;
+      red[1][warp] = Sw;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (warp == 0) {
-    const float m_in = lane < NW ? red[0][lane] : kNegInit * kLog2e;
-    const float M = warp_max(m_in);
-    const float S = warp_sum(lane < NW ? red[1][lane] * ex2f(m_in - M) : 0.f);
+    float M = Mw, S = Sw;
+    if (NW > 1) {
+      const float m_in = lane < NW ? red[0][lane] : kNegInit * kLog2e;
+      M = warp_max(m_in);
+      S = warp_sum(lane < NW ? red[1][lane] * ex2f(m_in - M) : 0.f);
+    }
     if (lane == 0) {
       p.stats[n * p.splits + k] = make_float2(M, S);
       int64_t c = p.ids[b * p.ids_stride + t];
@@ -377,10 +388,12 @@ __global__ void __launch_bounds__(kPairThreads) pref_loss_kernel(const Params p)
 // Gradient of one row (or its split); rows without a coefficient are written as zeros and not read.  Taking the rows in
 // the opposite order of the forward sweep, with or without L2 policies that keep its last 32 MB, changed nothing
 // measurable (229 us against 228 for 4 x 256 pairs at 151936 columns).
-template <int THREADS, int UNROLL, bool CAP, bool SCALAR>
-__global__ void __launch_bounds__(THREADS) pref_dlogits_kernel(const Params p) {
-  const int64_t r = blockIdx.x / unsigned(p.splits);
-  const int k = int(blockIdx.x - r * p.splits);
+template <int THREADS, int ROWS, int UNROLL, bool CAP, bool SCALAR>
+__global__ void __launch_bounds__(THREADS * ROWS) pref_dlogits_kernel(const Params p) {
+  const unsigned item = ROWS > 1 ? blockIdx.x * ROWS + threadIdx.y : blockIdx.x;
+  if (ROWS > 1 && item >= unsigned(2 * p.n_pairs * p.seq_rows)) return;
+  const int64_t r = item / unsigned(p.splits);
+  const int k = int(item - r * p.splits);
   const int64_t b = r / p.seq_rows, t = r - b * p.seq_rows;
   const int64_t c0 = int64_t(k) * p.split_cols;
   const int64_t V = p.vocab - c0 < p.split_cols ? p.vocab - c0 : p.split_cols;
@@ -433,18 +446,28 @@ static cudaError_t launch_pairs(const Params& p, cudaStream_t s) {
   return done();
 }
 
+// Short rows are a warp's each: 26 x 773 rows of 231 columns 32 us, with a CTA each 50; 32 x 512 of 2048 40 and 47, of
+// 4096 67 and 63.
+static bool warp_rows(const Params& p) { return p.splits == 1 && p.vocab <= kWarpCols; }
+
 static cudaError_t launch_forward(const Params& p, cudaStream_t s) {
   const unsigned grid = unsigned(2 * p.n_pairs * p.scored_rows * p.splits);
   const bool cap = p.softcap > 0.f, small = p.split_cols <= 16384;
-  if (small) {
+  if (warp_rows(p)) {
+    const unsigned ctas = (grid + kRowsPerCta - 1) / kRowsPerCta;
     if (cap)
-      pref_stats_kernel<128, 4, true><<<grid, 128, 0, s>>>(p);
+      pref_stats_kernel<32, kRowsPerCta, 4, true><<<ctas, dim3(32, kRowsPerCta), 0, s>>>(p);
     else
-      pref_stats_kernel<128, 4, false><<<grid, 128, 0, s>>>(p);
+      pref_stats_kernel<32, kRowsPerCta, 4, false><<<ctas, dim3(32, kRowsPerCta), 0, s>>>(p);
+  } else if (small) {
+    if (cap)
+      pref_stats_kernel<128, 1, 4, true><<<grid, 128, 0, s>>>(p);
+    else
+      pref_stats_kernel<128, 1, 4, false><<<grid, 128, 0, s>>>(p);
   } else if (cap) {
-    pref_stats_kernel<512, 4, true><<<grid, 512, 0, s>>>(p);
+    pref_stats_kernel<512, 1, 4, true><<<grid, 512, 0, s>>>(p);
   } else {
-    pref_stats_kernel<512, 4, false><<<grid, 512, 0, s>>>(p);
+    pref_stats_kernel<512, 1, 4, false><<<grid, 512, 0, s>>>(p);
   }
   cudaError_t e = done();
   if (e != cudaSuccess) return e;
@@ -452,10 +475,10 @@ static cudaError_t launch_forward(const Params& p, cudaStream_t s) {
 }
 
 template <typename K>
-static cudaError_t launch_rows(K* kernel, const Params& p, unsigned grid, unsigned threads, bool beside, cudaStream_t s) {
+static cudaError_t launch_rows(K* kernel, const Params& p, unsigned grid, dim3 threads, bool beside, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = threads;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -469,9 +492,13 @@ static cudaError_t launch_rows(K* kernel, const Params& p, unsigned grid, unsign
 
 template <bool CAP>
 static cudaError_t launch_backward_t(const Params& p, unsigned grid, bool same_phase, bool beside, cudaStream_t s) {
-  if (!same_phase) return launch_rows(pref_dlogits_kernel<256, 4, CAP, true>, p, grid, 256, beside, s);
-  if (p.split_cols <= 16384) return launch_rows(pref_dlogits_kernel<128, 4, CAP, false>, p, grid, 128, beside, s);
-  return launch_rows(pref_dlogits_kernel<512, 4, CAP, false>, p, grid, 512, beside, s);
+  if (!same_phase) return launch_rows(pref_dlogits_kernel<256, 1, 4, CAP, true>, p, grid, 256, beside, s);
+  if (warp_rows(p)) {
+    const unsigned ctas = (grid + kRowsPerCta - 1) / kRowsPerCta;
+    return launch_rows(pref_dlogits_kernel<32, kRowsPerCta, 4, CAP, false>, p, ctas, dim3(32, kRowsPerCta), beside, s);
+  }
+  if (p.split_cols <= 16384) return launch_rows(pref_dlogits_kernel<128, 1, 4, CAP, false>, p, grid, 128, beside, s);
+  return launch_rows(pref_dlogits_kernel<512, 1, 4, CAP, false>, p, grid, 512, beside, s);
 }
 
 // beside: right behind launch_forward, whose last launch it need not wait for as a whole.

@@ -343,3 +343,15 @@ def test_captured_backward(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(loss.detach(), want[k][0]) and torch.equal(grad, want[k][1])
+
+
+@pytest.mark.parametrize("P,T,V,kw", [(1, 3, 1, {}), (7, 61, 2047, dict(loss_type="ipo")), (3, 50, 2048, {}), (3, 50, 2049, {}),
+                                      (2, 17, 900, dict(softcap=30.0))])
+def test_short_rows(cuda, P, T, V, kw):
+    """Rows of a warp each, to the last that is and the first that is not; rows behind the scored ones."""
+    logits, ids, mask, rf = _case(P, T, V, P + T + V, cuda)
+    cfg = G.PreferenceConfig(**kw)
+    _check(G.preference_value_and_grad(logits, ids, mask, rf, cfg=cfg), logits, ids, mask, rf, cfg)
+    if T > 3:
+        out = G.preference_value_and_grad(logits, ids, mask, rf[:, 1:], shifted=True, cfg=cfg)
+        _check(out, logits, ids[:, 1:], mask[:, 1:], rf[:, 1:], cfg, scored=T - 1)
