@@ -138,7 +138,7 @@ constexpr int kRowsPerCta = 8;
 
 // One CTA (warp) per (scored row, split).  Bound by reading the unmasked rows once.
 template <int THREADS, int ROWS, int UNROLL, bool CAP>
-__global__ void __launch_bounds__(THREADS * ROWS) pref_stats_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS * ROWS, ROWS > 1 ? 5 : 0) pref_stats_kernel(const Params p) {
   constexpr int NW = THREADS / 32;
   __shared__ float red[2][NW];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kPairThreads) pref_loss_kernel(const Params p)
 // the opposite order of the forward sweep, with or without L2 policies that keep its last 32 MB, changed nothing
 // measurable (229 us against 228 for 4 x 256 pairs at 151936 columns).
 template <int THREADS, int ROWS, int UNROLL, bool CAP, bool SCALAR>
-__global__ void __launch_bounds__(THREADS * ROWS) pref_dlogits_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS * ROWS, ROWS > 1 ? 5 : 0) pref_dlogits_kernel(const Params p) {
   const unsigned item = ROWS > 1 ? blockIdx.x * ROWS + threadIdx.y : blockIdx.x;
   if (ROWS > 1 && item >= unsigned(2 * p.n_pairs * p.seq_rows)) return;
   const int64_t r = item / unsigned(p.splits);
@@ -446,7 +446,7 @@ static cudaError_t launch_pairs(const Params& p, cudaStream_t s) {
   return done();
 }
 
-// Short rows are a warp's each: 26 x 773 rows of 231 columns 32 us, with a CTA each 50; 32 x 512 of 2048 40 and 47, of
+// Short rows are a warp's each: 26 x 773 rows of 231 columns 30 us, with a CTA each 50; 32 x 512 of 2048 39 and 47, of
 // 4096 67 and 63.
 static bool warp_rows(const Params& p) { return p.splits == 1 && p.vocab <= kWarpCols; }
 
