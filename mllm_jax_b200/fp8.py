@@ -107,6 +107,26 @@ def _bind(x: Fp8Blocks, w: Fp8Blocks) -> _lib.Fp8Args:
                         hidden_scales=x.scales.data_ptr(), weight=w_at, weight_scales=w.scales.data_ptr())
 
 
+def _quantize_and_bind(x: torch.Tensor, w: Fp8Blocks, room: int) -> Tuple[_lib.Fp8Args, torch.Tensor, int]:
+    """Rows x [M, K] quantised into one buffer and bound with w; the buffer has `room` more bytes from the returned place
+    on (16-byte aligned).  One allocation: a small call is bound by the host."""
+    N, K, w_stride, w_at = _operand(w, "w", (BLOCK, BLOCK))
+    M, dev = x.shape[0], x.device
+    if dev != w.device or x.shape[1] != K or N < 1:
+        raise ValueError(f"x {tuple(x.shape)} on {dev} and w {tuple(w.shape)} on {w.device} do not match")
+    if x.stride(1) != 1 or (M > 1 and x.stride(0) < K):
+        x = x.contiguous()
+    scales = M * K
+    end = scales + (4 * M * -(-K // BLOCK) + 15) // 16 * 16
+    buf = torch.empty(end + room, dtype=torch.uint8, device=dev)
+    at = buf.data_ptr()
+    _lib.launch("mllm_lm_head_fp8_quantize", _lib.Fp8QuantizeArgs(
+        rows=M, cols=K, x_stride=x.stride(0) if M > 1 else K, q_stride=K, block_rows=1, dtype=_DTYPES[x.dtype],
+        x=x.data_ptr(), q=at, scales=at + scales), dev)
+    return _lib.Fp8Args(n_rows=M, vocab=N, hidden_dim=K, hidden_stride=K, weight_stride=w_stride, hidden=at,
+                        hidden_scales=at + scales, weight=w_at, weight_scales=w.scales.data_ptr()), buf, end
+
+
 def fp8_matmul(x: Union[Fp8Blocks, torch.Tensor], w: Fp8Blocks, *, out_dtype: torch.dtype = torch.bfloat16,
                out: Optional[torch.Tensor] = None, device_status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [M, K] (Fp8Blocks with blocks of (1, 128), or a tensor, which is quantised first) times w [N, K] (blocks of

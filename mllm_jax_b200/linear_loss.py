@@ -23,7 +23,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .fp8 import Fp8Blocks, _bind, quantize_fp8
+from .fp8 import Fp8Blocks, _quantize_and_bind
 from .ops import LossConfig, TokenLossProblem
 
 
@@ -82,9 +82,11 @@ def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]
     N = B * T
     lib = _lib.load()
     if fp8:
-        hq = quantize_fp8(hidden.reshape(N, H), block=(1, 128))
-        a = _bind(hq, weight)
         splits, nbytes = 1, int(lib.mllm_lm_head_fp8_partials_bytes(N, V))
+        # the quantised rows, then the partials (unless the caller has room for them) and a status word
+        a, hq, place = _quantize_and_bind(hidden.reshape(N, H), weight, 16 + (nbytes if workspace is None else 0))
+        if workspace is None:
+            workspace = hq[place + 16:]
     else:
         a = _lib.LmHeadArgs()
         splits = int(lib.mllm_lm_head_splits(N, V))
@@ -96,7 +98,7 @@ def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]
     forward_only = advantages is None
     if fp8 and forward_only and group is None and vocab_start == 0 and vocab_total in (None, V) and \
             total_valid_token_count is None and old_per_token_logps is None and ref_per_token_logps is None:
-        return _fp8_logprobs(a, hq, weight, token_ids, cfg, workspace, B, T, dev)
+        return _fp8_logprobs(a, hq, place, weight, token_ids, cfg, workspace, B, T, dev)
     if forward_only:
         advantages = torch.zeros(B, dtype=torch.float32, device=dev)
     # side arrays, outputs and residuals exactly as for materialised logits; no logits tensor is bound
@@ -140,11 +142,15 @@ def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]
 class _LogprobsCall:
     """What a log-probs-only call keeps alive, and its status word."""
 
-    def __init__(self, device_status, *keep):
-        self.device_status, self._keepalive = device_status, keep
+    def __init__(self, buffer, place, *keep):
+        self._buffer, self._place, self._keepalive = buffer, place, keep
+
+    @property
+    def device_status(self) -> torch.Tensor:
+        return self._buffer[self._place:self._place + 4].view(torch.int32)
 
 
-def _fp8_logprobs(a, hq: Fp8Blocks, weight: Fp8Blocks, token_ids, cfg: LossConfig, workspace, B: int, T: int, dev) -> dict:
+def _fp8_logprobs(a, hq: torch.Tensor, place: int, weight: Fp8Blocks, token_ids, cfg: LossConfig, workspace, B: int, T: int, dev) -> dict:
     """Log-probs, entropies and log-sum-exps of an unsharded 8-bit head: three launches, the last of which merges the
     vocabulary ranges and writes the results."""
     if token_ids.numel() != B * T:
@@ -152,17 +158,16 @@ def _fp8_logprobs(a, hq: Fp8Blocks, weight: Fp8Blocks, token_ids, cfg: LossConfi
     if token_ids.dtype is torch.int64:
         token_ids = token_ids.clamp(-1, 2 ** 31 - 1)  # an id beyond 32 bits must not wrap to a valid one
     ids = token_ids.to(device=dev, dtype=torch.int32).contiguous()
-    status = torch.empty(1, dtype=torch.int32, device=dev)
     out = torch.empty(3, B, T, dtype=torch.float32, device=dev)
     lp, ent, lse = out.unbind(0)
-    a.chosen_ids, a.partials, a.call_status = ids.data_ptr(), workspace.data_ptr(), status.data_ptr()
+    a.chosen_ids, a.partials, a.call_status = ids.data_ptr(), workspace.data_ptr(), hq.data_ptr() + place
     a.softcap, a.temperature = float(cfg.softcap) if cfg.softcap else 0.0, cfg.temperature
     a.per_token_logps, a.lse = lp.data_ptr(), lse.data_ptr()
     if cfg.compute_entropy:
         a.token_entropy = ent.data_ptr()
     _lib.launch("mllm_lm_head_fp8_partials", a, dev)
     return {"per_token_logps": lp, "token_entropy": ent if cfg.compute_entropy else None, "lse": lse,
-            "problem": _LogprobsCall(status, hq, weight, ids, workspace), "splits": 1}
+            "problem": _LogprobsCall(hq, place, weight, ids, workspace), "splits": 1}
 
 
 def linear_grpo_value_and_grad(hidden: torch.Tensor, weight: torch.Tensor, token_ids: torch.Tensor,

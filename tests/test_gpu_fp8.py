@@ -320,3 +320,28 @@ def test_call_status_beside_a_running_one(cuda):
         a.chosen_ids = chosen.data_ptr()
         _lib.launch("mllm_lm_head_fp8_partials", a, x.device)
         assert int(mine) == bits and int(running) == total
+
+
+def test_folded_head_workspaces_and_refusals(cuda):
+    from mllm_jax_b200 import _lib
+    B, T, H, V = 2, 9, 48, 500
+    wide = _x(B * T, 2 * H, torch.bfloat16, 103, cuda).view(B, T, 2 * H)
+    w = G.quantize_fp8(_x(V, H, torch.bfloat16, 104, cuda), block=(128, 128))
+    ids = torch.randint(0, V, (B, T), generator=torch.Generator().manual_seed(105)).to(cuda)
+    want = lm_head_forward(wide[..., :H].contiguous(), w, ids)
+    room = torch.full((_lib.load().mllm_lm_head_fp8_partials_bytes(B * T, V) + 32,), 9, dtype=torch.uint8, device=cuda)
+    for hidden, kw in ((wide[..., :H], {}), (wide[..., :H].transpose(1, 2).contiguous().transpose(1, 2), {}),
+                       (wide[..., :H], dict(workspace=room[:-32]))):
+        got = lm_head_forward(hidden, w, ids, **kw)
+        for k in ("per_token_logps", "token_entropy", "lse"):
+            assert torch.equal(got[k], want[k])
+        assert int(got["problem"].device_status) == 0
+    assert bool((room[-32:] == 9).all())
+    with pytest.raises(ValueError, match="multiple of 16"):
+        lm_head_forward(wide[..., :40], G.quantize_fp8(_x(V, 40, torch.bfloat16, 104, cuda), block=(128, 128)), ids)
+    with pytest.raises(ValueError, match="workspace"):
+        lm_head_forward(wide[..., :H], w, ids, workspace=room[:64])
+    with pytest.raises(ValueError, match="blocks"):
+        lm_head_forward(wide[..., :H], G.quantize_fp8(_x(V, H, torch.bfloat16, 104, cuda)), ids)
+    with pytest.raises(ValueError, match="do not match"):
+        lm_head_forward(wide, w, ids)
