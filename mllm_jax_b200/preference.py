@@ -146,6 +146,16 @@ class PreferenceProblem:
                 "rejected_logps": bad_lp}
 
 
+def _shifted(t: torch.Tensor, B: int, L: int, name: str) -> torch.Tensor:
+    if t.shape != (B, L):
+        raise ValueError(f"{name} must have shape {(B, L)}, got {tuple(t.shape)}")
+    return t.narrow(1, 1, L - 1) if L > 1 else t[:, 1:]
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device)
+
+
 def _from_logits(logits, token_ids, mask, ref, shifted, cfg, pair_weights, total_pairs) -> PreferenceProblem:
     if not logits.is_cuda:
         raise RuntimeError("the preference loss kernels run on a CUDA device only (no CPU path)")
@@ -158,7 +168,7 @@ def _from_logits(logits, token_ids, mask, ref, shifted, cfg, pair_weights, total
     if V < 1 or (V > 1 and logits.stride(2) != 1) or row < V or logits.stride(0) != L * row:
         raise ValueError("logits must have unit stride on the vocabulary and rows evenly spaced")
     if shifted:
-        token_ids, mask = token_ids[:, 1:], None if mask is None else mask[:, 1:]
+        token_ids, mask = _shifted(token_ids, B, L, "token ids"), None if mask is None else _shifted(mask, B, L, "mask")
     T = L - 1 if shifted else L
     prob = PreferenceProblem(B, T, logits.device, mask, ref, pair_weights, total_pairs, cfg or PreferenceConfig())
     prob.bind_logits(logits, token_ids, L, row)
@@ -183,8 +193,7 @@ def preference_value_and_grad(logits: torch.Tensor, token_ids: torch.Tensor, mas
     prob.a.grad_scale = float(grad_scale)
     given = inplace or dlogits is not None
     if dlogits is None:
-        dlogits = logits if inplace else torch.empty_strided(logits.shape, logits.stride(), dtype=logits.dtype,
-                                                             device=logits.device)
+        dlogits = logits if inplace else _like(logits)
     prob.bind_dlogits(dlogits)
     prob.run("mllm_grpo_preference_fwd_bwd")
     if given:
@@ -215,8 +224,7 @@ class _PreferenceLoss(torch.autograd.Function):
         logits = ctx.saved_tensors[0]
         scale = grad_loss.to(torch.float32).reshape(1).contiguous()
         prob.a.grad_scale_dev = scale.data_ptr()
-        prob.bind_dlogits(logits if ctx.inplace else torch.empty_strided(
-            logits.shape, logits.stride(), dtype=logits.dtype, device=logits.device))
+        prob.bind_dlogits(logits if ctx.inplace else _like(logits))
         prob.run("mllm_grpo_preference_bwd")
         if ctx.inplace:
             _lib.written(logits)  # another backward that needs what they held is an error
