@@ -287,3 +287,73 @@ def test_grad_into_strided_rows(cuda, N, H, stride, offset, out_dtype):
     ref, mag, n = _grad_ref(x, ids.long(), V, 1.0)
     R.assert_within(rows[:, :H], ref, _grad_bound(ref, mag, n, out_dtype), "dweight")
     assert bool((rows[:, H:] == 7).all()) and bool((buf[:offset] == 7).all()) and bool((buf[offset + V * stride:] == 7).all())
+
+
+@pytest.mark.parametrize("N", [5, 1100])
+def test_grad_in_several_fills(cuda, N):
+    """More than 2^31 words of two bytes, in rows some distance apart at an odd address, so that zeros go out an element at
+    a time in several launches: all of them beside the sort, or (more tokens) most behind it."""
+    from mllm_jax_b200 import _lib
+    V, H, stride = 70001, 32769, 32771
+    per_launch = 2 ** 31 // H
+    gen = torch.Generator().manual_seed(20)
+    ids = torch.randperm(V, generator=gen)[:N]
+    first = 0 if N == 5 else ((128 << 20) + N * 4096) // (H * 2) + 1   # rows whose zeros are written beside the sort
+    assert (N * H * 2 > 64 << 20) == (first > 0)
+    edges = torch.tensor([per_launch - 1, per_launch, V - 1, 0] if N == 5 else
+                         [first - 1, first, first + per_launch - 1, first + per_launch, V - 1, 0])
+    ids = torch.cat([ids[~torch.isin(ids, edges)][:N - len(edges)], edges]).to(cuda)
+    x = _rows(ids.numel(), H, torch.float16, 20, cuda)
+    buf = torch.full((1 + V * stride,), 7.0, dtype=torch.float16, device=cuda)
+    a = _lib.EmbeddingArgs()
+    n = ids.numel()
+    a.n_tokens, a.vocab, a.hidden, a.weight_stride, a.token_stride, a.scale = n, V, H, stride, H, 1.0
+    a.dtype = a.out_dtype = _lib.DTYPE_F16
+    work = torch.empty(_lib.load().mllm_grpo_embedding_workspace_bytes(n, H, V), dtype=torch.uint8, device=cuda)
+    ids32 = ids.to(torch.int32)
+    a.ids, a.grad_out, a.workspace, a.dweight = ids32.data_ptr(), x.data_ptr(), work.data_ptr(), buf.data_ptr() + 2
+    _lib.launch("mllm_grpo_embedding_grad", a, x.device)
+    rows = buf[1:].view(V, stride)
+    assert torch.equal(rows[ids, :H], x)
+    rows[ids, :H] = 0
+    assert not any(part.any() for part in rows[:, :H].split(4096))
+    assert bool((rows[:, H:] == 7).all()) and float(buf[0]) == 7
+
+
+@pytest.mark.parametrize("N", [65537, 131072, 200003])
+@pytest.mark.parametrize("V", [300, 100000, 300000])   # one, two and three digits
+@pytest.mark.parametrize("kind", ["any", "one", "pad"])
+def test_grad_of_many_tokens(cuda, N, V, kind):
+    """More than 65536 tokens: a CTA of the sort has several tiles."""
+    gen = torch.Generator().manual_seed(N + V)
+    ids = torch.randint(0, V, (N,), generator=gen)
+    if kind == "one":
+        ids[:] = V - 1
+    elif kind == "pad":
+        ids[N // 3:] = 17
+        ids[5], ids[N - 1] = V - 1, 0
+    ids = ids.to(cuda)
+    x = _rows(N, 16, torch.bfloat16, N, cuda)
+    out = G.embedding_grad(x, ids, V)
+    ref, mag, n = _grad_ref(x, ids, V, 1.0)
+    R.assert_within(out, ref, _grad_bound(ref, mag, n, torch.float32), "dweight")
+    assert torch.equal(out, G.embedding_grad(x, ids, V))
+
+
+@pytest.mark.parametrize("H,dtype", [(4096, torch.bfloat16), (1030, torch.bfloat16), (1028, torch.float32), (1033, torch.float16)])
+def test_grad_added_to_many_heavy_rows(cuda, H, dtype):
+    """Sums added to a table whose rows have tens of tokens each, its columns in several parts."""
+    N, V = 20011, 431
+    gen = torch.Generator().manual_seed(21)
+    ids = (torch.rand(N, generator=gen) ** 2 * (V - 3)).long()   # a few hundred rows, the last three without tokens
+    ids[4000:7000] = 11
+    ids = ids.to(cuda)
+    x = _rows(N, H, dtype, 21, cuda)
+    base = _rows(V, H, torch.float32, 22, cuda)
+    out = base.clone()
+    assert G.embedding_grad(x, ids, V, scale=1.5, out=out) is out
+    ref, mag, n = _grad_ref(x, ids, V, 1.5)
+    assert int((n > 16).sum()) > 200
+    R.assert_within(out, base.double() + ref, _grad_bound(ref, mag, n, torch.float32) + 2.0 ** -23 * (base.double().abs() + ref.abs()), "accumulated")
+    assert torch.equal(out[V - 3:], base[V - 3:])
+    R.assert_within(G.embedding_grad(x, ids, V, scale=1.5), ref, _grad_bound(ref, mag, n, torch.float32), "new")

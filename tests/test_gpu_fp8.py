@@ -345,3 +345,124 @@ def test_folded_head_workspaces_and_refusals(cuda):
         lm_head_forward(wide[..., :H], G.quantize_fp8(_x(V, H, torch.bfloat16, 104, cuda)), ids)
     with pytest.raises(ValueError, match="do not match"):
         lm_head_forward(wide, w, ids)
+
+
+@pytest.mark.parametrize("M,N,K", [(2050, 300, 272), (4200, 300, 144), (4200, 1500, 272), (2305, 2200, 128)])
+def test_product_of_many_rows(cuda, M, N, K):
+    """More than 2048 rows: several groups of row tiles, the last of them shorter; an odd number of row tiles for pairs."""
+    x, w = _operands(M, N, K, M + N, cuda)
+    ref, mag = R.product(x.values, x.scales, w.values, w.scales)
+    for out_dtype in (torch.float32, torch.bfloat16):
+        out = G.fp8_matmul(x, w, out_dtype=out_dtype)
+        R.assert_within(out, ref, R.product_bound(ref, mag, K) + ref.abs() * R.HALF_STEP[out_dtype] + R.TINY_STEP[out_dtype], f"{M}x{N}x{K}")
+
+
+# rows, width, columns, tiles of 256 columns in a range
+LONG_HEADS = [(70, 64, 40000, 2), (128, 80, 76801, 3), (300, 48, 40000, 5), (2300, 64, 2000, None)]
+
+
+@pytest.mark.parametrize("N,H,V,per", LONG_HEADS)
+@pytest.mark.parametrize("cap", [None, 30.0])
+def test_folded_head_of_several_tiles_per_range(cuda, N, H, V, per, cap):
+    """Ranges of several tiles and a shorter last one, with logits that rise from tile to tile for half of the rows and
+    fall for the other half, chosen columns in first and last tiles; more rows than one group of row tiles."""
+    from mllm_jax_b200 import _lib
+    tiles = -(-V // 256)
+    if per is not None:
+        entries = _lib.load().mllm_lm_head_fp8_partials_bytes(N, V) // (16 * N) - 1
+        assert entries == 2 * -(-tiles // per) and tiles % per, "the case is meant for another plan"
+    g = torch.Generator().manual_seed(N + V)
+    side = torch.where(torch.arange(N) % 2 == 0, 1.0, -1.0)[:, None]
+    hidden = torch.randn(N, H, generator=g)
+    hidden[:, :16] = side
+    wt = torch.randn(V, H, generator=g) * 2 / H ** 0.5
+    wt[:, :16] = 0.6 * torch.arange(V)[:, None] / V          # +- 9.6 from the first column to the last
+    hidden, w = hidden.to(torch.bfloat16).to(cuda), G.quantize_fp8(wt.to(cuda), block=(128, 128))
+    ids = torch.randint(0, V, (N,), generator=g, dtype=torch.int32)
+    edges = [0, V - 1, 255, 256, 511, 512, V - 257, (tiles - 1) * 256, V // 2, 1279, 1280]
+    ids[:len(edges)] = torch.tensor(edges, dtype=torch.int32)
+    ids = ids.to(cuda)
+    out = lm_head_forward(hidden, w, ids, cfg=G.LossConfig(softcap=cap))
+    torch.cuda.synchronize()
+    assert G.ops.check_device_status(out["problem"]) == 0
+    q = G.quantize_fp8(hidden)
+    y, mag = R.product(q.values, q.scales, w.values, w.scales)
+    worst = R.product_bound(y, mag, H).amax(1)
+    if cap:
+        y, worst = cap * torch.tanh(y / cap), worst + 2.6e-7 * cap
+    lse = torch.logsumexp(y, 1)
+    lp = y.gather(1, ids.long()[:, None])[:, 0] - lse
+    p = torch.exp(y - lse[:, None])
+    ent = -(p * (y - lse[:, None])).sum(1)
+    # a term's exponent is rounded twice (2^-19 each while |y log2e| <= 64), ex2.approx is off by 2^-22; a thread adds up
+    # 64 terms of a tile in each of two sums, and fewer than 600 additions in f32 follow from the tiles and ranges; every
+    # further tile may raise the maximum, where the sum is multiplied by an ex2.approx (2^-22) of a rounded exponent a
+    # (2^-23 a of a weight 2^-a: at most 2^-23) and rounded; logarithm, merged maximum and result are below 64 in f32
+    e_sum = 3 * 2.0 ** -20 + 2.0 ** -22 + 664 * 2.0 ** -24 + (per or 8) * 2.0 ** -21 + 4 * 2.0 ** -19
+    R.assert_within(out["lse"].view(-1), lse, worst + e_sum, "lse")
+    R.assert_within(out["per_token_logps"].view(-1), lp, 2 * worst + e_sum, "log-probs")
+    R.assert_within(out["token_entropy"].view(-1), ent, 2 * worst * (1 + y.abs().amax(1)) + e_sum * (2 + (p * y.abs()).sum(1)), "entropy")
+
+
+def _gathered(monkeypatch, ranks, record):
+    """all_gather_into_tensor of `ranks` ranks in one process: records what this call sends, or hands out what each sent."""
+    import torch.distributed as dist
+
+    def gather(parts, mine, group=None):
+        if ranks == 1:
+            record.append(mine.clone())
+            parts.copy_(mine)
+        else:
+            torch.cat(record, out=parts)
+
+    monkeypatch.setattr(dist, "get_world_size", lambda group=None: ranks)
+    monkeypatch.setattr(dist, "all_gather_into_tensor", gather)
+
+
+@pytest.mark.parametrize("cap", [None, 25.0])
+def test_folded_head_over_a_group(cuda, monkeypatch, cap):
+    """The group branch with an 8-bit weight: the merged records of two vocabulary shards, gathered rank by rank, give
+    the log-probs, entropies, log-sum-exps and the loss of the whole head."""
+    B, T, H, V, cut = 2, 33, 64, 2304, 896
+    g = torch.Generator().manual_seed(110)
+    hidden = torch.randn(B, T, H, generator=g).to(torch.bfloat16).to(cuda)
+    w = G.quantize_fp8((torch.randn(V, H, generator=g) * 0.4).to(cuda), block=(128, 128))
+    shards = [(0, G.Fp8Blocks(w.values[:cut], w.scales[:cut // 128])), (cut, G.Fp8Blocks(w.values[cut:], w.scales[cut // 128:]))]
+    ids = torch.randint(0, V, (B, T), generator=g).to(cuda)
+    ids[0, :4] = torch.tensor([0, cut - 1, cut, V - 1])
+    mask, adv = torch.ones(B, T, device=cuda), torch.randn(B, generator=g).to(cuda)
+    cfg = G.LossConfig(softcap=cap)
+    want = lm_head_forward(hidden, w, ids, mask, adv, cfg=cfg)
+    sent, group = [], object()
+    _gathered(monkeypatch, 1, sent)
+    for start, shard in shards:
+        lm_head_forward(hidden, shard, ids, mask, adv, cfg=cfg, vocab_start=start, vocab_total=V, group=group)
+    assert [t.numel() for t in sent] == [16 * B * T] * 2
+    _gathered(monkeypatch, 2, sent)
+    for start, shard in shards:
+        for extra in ((mask, adv), ()):
+            out = lm_head_forward(hidden, shard, ids, *extra, cfg=cfg, vocab_start=start, vocab_total=V, group=group)
+            assert G.ops.check_device_status(out["problem"]) == 0
+            # the same f32 tile sums, merged in another order: a few roundings of numbers below 64
+            for k in ("per_token_logps", "token_entropy", "lse"):
+                R.assert_within(out[k], want[k].double(), 6 * 2.0 ** -18, k)
+            if extra:
+                R.assert_within(out["loss"], want["loss"].double(), 2.0 ** -17 * (1 + float(adv.abs().max())), "loss")
+
+
+def test_folded_head_over_a_process_group_of_one(cuda, tmp_path):
+    import torch.distributed as dist
+
+    B, T, H, V = 1, 20, 32, 700
+    hidden = _x(T, H, torch.bfloat16, 111, cuda).view(B, T, H)
+    w = G.quantize_fp8(_x(V, H, torch.bfloat16, 112, cuda), block=(128, 128))
+    ids = torch.randint(0, V, (B, T), generator=torch.Generator().manual_seed(113)).to(cuda)
+    want = lm_head_forward(hidden, w, ids, advantages=torch.zeros(B, device=cuda))
+    dist.init_process_group("nccl", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        out = lm_head_forward(hidden, w, ids, group=dist.group.WORLD)
+        torch.cuda.synchronize()
+    finally:
+        dist.destroy_process_group()
+    for k in ("per_token_logps", "token_entropy", "lse"):
+        assert torch.equal(out[k], want[k])

@@ -355,3 +355,41 @@ def test_short_rows(cuda, P, T, V, kw):
     if T > 3:
         out = G.preference_value_and_grad(logits, ids, mask, rf[:, 1:], shifted=True, cfg=cfg)
         _check(out, logits, ids[:, 1:], mask[:, 1:], rf[:, 1:], cfg, scored=T - 1)
+
+
+def _large_case(P, T, V, seed, device):
+    """As `_case` with reference log-probs per token, made on the device and a sequence at a time."""
+    g = torch.Generator(device).manual_seed(seed)
+    B = 2 * P
+    logits = torch.empty(B, T, V, dtype=torch.bfloat16, device=device)
+    ids = torch.randint(0, V, (B, T), generator=g, dtype=torch.int32, device=device)
+    rf = torch.empty(B, T, device=device)
+    for b in range(B):
+        logits[b] = 2 * torch.randn(T, V, generator=g, device=device)
+        lp = torch.log_softmax(logits[b].double(), -1).gather(-1, ids[b].long()[:, None])[:, 0]
+        rf[b] = lp + 0.5 * torch.randn(T, generator=g, device=device)
+    end = torch.randint(max(1, T // 2), T + 1, (B, 1), generator=g, device=device)
+    at = torch.arange(T, device=device)[None]
+    return logits, ids, ((at < end) & (at >= T // 4)).to(torch.int32), rf
+
+
+@pytest.mark.parametrize("P,T,V,kw", [
+    (37, 64, 16501, {}), (37, 64, 16501, dict(softcap=30.0, average=True)),                  # 4736 tokens: rows unsplit
+    (37, 32, 33001, dict(loss_type="ipo")), (37, 32, 33001, dict(softcap=30.0)),             # two parts of 16504 columns
+    (5, 158, 50001, dict(label_smoothing=0.1)), (5, 158, 50001, dict(softcap=20.0, loss_type="hinge")),  # three of 16672
+])
+def test_parts_of_more_than_16384_columns(cuda, P, T, V, kw):
+    """So many tokens that a row, or its part, is too long for the CTAs of 128 threads: those of 512 take it."""
+    cfg = G.PreferenceConfig(**kw)
+    logits, ids, mask, rf = _large_case(P, T, V, P + T + V, cuda)
+    ids[0, T // 4], ids[0, T // 4 + 1], ids[1, T // 4], ids[1, T // 4 + 1] = 0, V - 1, 16503 % V, 16504 % V
+    out = G.preference_value_and_grad(logits, ids, mask, rf, cfg=cfg)
+    torch.cuda.synchronize()
+    assert int(out["problem"].device_status.item()) == 0
+    _check(out, logits, ids, mask, rf, cfg)
+    if P == 5:  # rows behind the scored ones, and a gradient buffer of another phase than the logits
+        big = torch.full((2 * P * T * V + 8,), 7.0, dtype=torch.bfloat16, device=cuda)
+        d = big[1:1 + 2 * P * T * V].view(2 * P, T, V)
+        out = G.preference_value_and_grad(logits, ids, mask, rf[:, 1:], shifted=True, cfg=cfg, dlogits=d)
+        _check(out, logits, ids[:, 1:], mask[:, 1:], rf[:, 1:], cfg, scored=T - 1)
+        assert float(big[0]) == 7 and bool((big[1 + d.numel():] == 7).all())
