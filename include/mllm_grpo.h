@@ -375,7 +375,7 @@ typedef struct mllm_grpo_preference_args {
   void* workspace;         /* mllm_grpo_preference_workspace_bytes(...), 16-byte aligned; carries the residuals from
                               mllm_grpo_preference_fwd to mllm_grpo_preference_bwd */
   int32_t* device_status;  /* optional: MLLM_GRPO_DEV_* bits are ORed in */
-  int32_t* call_status;    /* optional: set to this call's MLLM_GRPO_DEV_* bits (forward from logits) */
+  int32_t* call_status;    /* optional: set to this call's MLLM_GRPO_DEV_* bits by a forward (from log-probs: 0) */
 } mllm_grpo_preference_args;
 
 /* Forward from logits: loss, rewards, sequence_logps and the residuals of the backward.  Rows with mask 0 are not read. */

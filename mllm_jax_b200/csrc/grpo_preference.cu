@@ -383,6 +383,7 @@ __global__ void __launch_bounds__(THREADS) pref_pairs_kernel(const Params p) {
 __global__ void __launch_bounds__(kPairThreads) pref_loss_kernel(const Params p) {
   __shared__ double red[32];
   reduce_loss(p, red);
+  if (threadIdx.x == 0 && p.call_status) *p.call_status = 0;  // no ids, nothing to raise
 }
 
 // Gradient of one row (or its split); rows without a coefficient are written as zeros and not read.  Taking the rows in

@@ -113,7 +113,7 @@ class PreferenceProblem:
 
     @property
     def device_status(self) -> torch.Tensor:
-        """MLLM_GRPO_DEV_* bits of the forward from logits (an int32 on the device)."""
+        """MLLM_GRPO_DEV_* bits of the forward (an int32 on the device; nothing raises one from log-probs)."""
         return self.out[-1:].view(torch.int32)
 
     def bind_logits(self, logits: torch.Tensor, ids: torch.Tensor, L: int, row_stride: int) -> None:

@@ -393,3 +393,16 @@ def test_parts_of_more_than_16384_columns(cuda, P, T, V, kw):
         out = G.preference_value_and_grad(logits, ids, mask, rf[:, 1:], shifted=True, cfg=cfg, dlogits=d)
         _check(out, logits, ids[:, 1:], mask[:, 1:], rf[:, 1:], cfg, scored=T - 1)
         assert float(big[0]) == 7 and bool((big[1 + d.numel():] == 7).all())
+
+
+def test_status_from_log_probs(cuda):
+    """A problem's status word says what its kernels raised, from log-probs as well: nothing, whatever lay in the
+    memory that the call was given."""
+    P, T = 5, 9
+    lp = -torch.rand(2 * P, T, device=cuda)
+    for form in (G.preference_logps_value_and_grad, G.preference_loss_from_logps):
+        dirty = [torch.full((2 + 4 * P,), -1, dtype=torch.int32, device=cuda) for _ in range(64)]
+        del dirty  # the next allocations of this size
+        out = form(lp, None)
+        torch.cuda.synchronize()
+        assert G.ops.check_device_status(out["problem"]) == 0
