@@ -236,6 +236,16 @@ def written(t) -> None:
         increment_version(t)
 
 
+def no_tangent(t, name: str) -> None:
+    """Refuses a forward-mode dual tensor: the kernels read its value by address and would drop its tangent."""
+    import torch
+
+    ad = torch.autograd.forward_ad
+    # outside of every dual level nothing carries one: 0.2 us, where unpacking takes 0.6 of a call of 10
+    if ad._current_level >= 0 and ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name} carries a forward-mode tangent, which the kernels do not propagate")
+
+
 def launch(name: str, args, device) -> None:
     """`call` on the current stream of `device` (a CUDA torch.device with an index), whichever device is current.
 

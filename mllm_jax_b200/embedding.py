@@ -86,13 +86,15 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 
                      vocab_total: Optional[int] = None, device_status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """ids [...] int32 / int64, weight [V, H] bf16 / f16 / f32 (rows any distance apart) -> [..., H] in weight's type.
 
-    Differentiable with respect to weight: its gradient is `embedding_grad` in weight's type, all [V, H] of it."""
+    Differentiable with respect to weight: its gradient is `embedding_grad` in weight's type, all [V, H] of it.  Reverse
+    mode only: a weight with a forward-mode tangent is refused."""
     if not weight.is_cuda:
         raise RuntimeError("embedding_lookup needs CUDA tensors: the kernels have no CPU path")
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"weight must be [V, H], got shape {tuple(weight.shape)}")
     if (weight.stride(1) != 1 and weight.shape[1] > 1) or (weight.shape[0] > 1 and weight.stride(0) < weight.shape[1]):
         raise ValueError("weight rows must be contiguous and must not overlap")
+    _lib.no_tangent(weight, "weight")
     if weight.requires_grad and torch.is_grad_enabled():
         return _EmbeddingLookup.apply(weight, ids, float(scale), vocab_start, vocab_total, device_status)
     return _lookup(ids, weight, scale, vocab_start, vocab_total, device_status)
@@ -111,6 +113,7 @@ def embedding_grad(grad_out: torch.Tensor, ids: torch.Tensor, vocab: int, *, sca
     dev = grad_out.device
     if grad_out.dim() < 1 or grad_out.shape[:-1] != ids.shape or grad_out.shape[-1] < 1:
         raise ValueError(f"grad_out {tuple(grad_out.shape)} must be ids {tuple(ids.shape)} with one more dimension")
+    _lib.no_tangent(grad_out, "grad_out")
     vocab = int(vocab)
     H = grad_out.shape[-1]
     g = _rows(grad_out, H)

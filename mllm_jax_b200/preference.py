@@ -220,6 +220,7 @@ class _PreferenceLoss(torch.autograd.Function):
         prob: PreferenceProblem = ctx.prob
         if ctx.spent:
             raise RuntimeError("the first backward has overwritten the logits (inplace_backward=True)")
+        _lib.no_tangent(grad_loss, "the loss's cotangent")
         ctx.spent = ctx.inplace
         logits = ctx.saved_tensors[0]
         scale = grad_loss.to(torch.float32).reshape(1).contiguous()

@@ -357,3 +357,28 @@ def test_grad_added_to_many_heavy_rows(cuda, H, dtype):
     R.assert_within(out, base.double() + ref, _grad_bound(ref, mag, n, torch.float32) + 2.0 ** -23 * (base.double().abs() + ref.abs()), "accumulated")
     assert torch.equal(out[V - 3:], base[V - 3:])
     R.assert_within(G.embedding_grad(x, ids, V, scale=1.5), ref, _grad_bound(ref, mag, n, torch.float32), "new")
+
+
+def test_forward_mode_tangents_are_refused(cuda):
+    """A tensor that carries a forward-mode tangent is an error, not a result that has lost it: in the lookup, with and
+    without gradients recorded, in its gradient, and in a backward pass whose cotangent has one."""
+    import torch.autograd.forward_ad as fwd
+
+    V, H = 11, 8
+    w, c = _rows(V, H, torch.float32, 30, cuda), _rows(5, H, torch.float32, 31, cuda)
+    ids = torch.tensor([0, 3, 3, 10, 7], device=cuda)
+    leaf = w.clone().requires_grad_(True)
+    out = G.embedding_lookup(ids, leaf)
+    with fwd.dual_level():
+        dual, cotangent = fwd.make_dual(w, torch.ones_like(w)), fwd.make_dual(c, torch.ones_like(c))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            G.embedding_lookup(ids, dual)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            G.embedding_lookup(ids, dual)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            G.embedding_grad(cotangent, ids, V)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(out, leaf, cotangent, retain_graph=True)
+        assert torch.equal(G.embedding_lookup(ids, w), w[ids])   # a tensor without one
+    (g,) = torch.autograd.grad(out, leaf, c)
+    assert torch.equal(g, G.embedding_grad(c, ids, V))

@@ -406,3 +406,30 @@ def test_status_from_log_probs(cuda):
         out = form(lp, None)
         torch.cuda.synchronize()
         assert G.ops.check_device_status(out["problem"]) == 0
+
+
+def test_forward_mode_cotangents_are_refused(cuda):
+    import torch.autograd.forward_ad as fwd
+
+    logits, ids, mask, rf = _case(1, 5, 40, 35, cuda)
+    x = logits.clone().requires_grad_(True)
+    loss = G.preference_loss(x, ids, mask, rf[:, 1:])["loss"]
+    lp = torch.full((2, 5), -1.0, device=cuda, requires_grad=True)
+    from_lp = G.preference_loss_from_logps(lp, mask, rf)["loss"]
+    one = torch.ones((), device=cuda)
+    with fwd.dual_level():
+        for out, leaf in ((loss, x), (from_lp, lp)):
+            dual = fwd.make_dual(one, one)
+            if leaf is x:
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    torch.autograd.grad(out, leaf, dual, retain_graph=True)
+            else:  # linear in the cotangent: its tangent comes through
+                (g,) = torch.autograd.grad(out, leaf, dual, retain_graph=True)
+                value, tangent = fwd.unpack_dual(g)
+                assert torch.equal(value, tangent)
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            G.preference_loss(fwd.make_dual(logits, torch.ones_like(logits)), ids, mask, rf[:, 1:])
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            G.preference_loss_from_logps(fwd.make_dual(lp.detach(), torch.ones_like(lp)), mask, rf)
+    (g,) = torch.autograd.grad(loss, x)
+    assert torch.isfinite(g).all() and g.any()

@@ -241,3 +241,14 @@ def test_written_tensors_change_their_version():
     assert t._version > before
     with torch.inference_mode():
         _lib.written(torch.zeros(3))
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+
+    t = torch.zeros(3)
+    _lib.no_tangent(t, "t")
+    with fwd.dual_level():
+        _lib.no_tangent(t, "t")
+        with pytest.raises(NotImplementedError, match="t carries a forward-mode tangent"):
+            _lib.no_tangent(fwd.make_dual(t, torch.ones(3)), "t")
