@@ -468,7 +468,12 @@ typedef struct mllm_lm_head_fp8_args {
   int32_t* device_status;     /* optional: MLLM_GRPO_DEV_* bits are ORed in */
   int32_t* call_status;       /* partials, optional: set to this call's bits */
 } mllm_lm_head_fp8_args;
+/* A wait inside the kernel that runs out (after 2 s) raises MLLM_GRPO_DEV_WAIT_TIMEOUT, and the elements of out that were
+ * not reached are NaN. */
 int mllm_lm_head_fp8_matmul(const mllm_lm_head_fp8_args* args, void* stream);
+/* Test hook: in calls that follow, each CTA (pair) stops multiplying after `tiles` output tiles as if an operand had
+ * never arrived, so that the waits for the next one run out; negative (the default): never. */
+void mllm_lm_head_fp8_stop_after(int32_t tiles);
 /* mllm_lm_head_partials with both operands in 8 bits.  The first n_rows records of `partials` are the rows' merged
  * (max, sumexp, sum e*y, chosen-or-0), to go through mllm_grpo_combine with n_shards = 1 (or, all-gathered over a
  * sharded head's ranks, n_shards = ranks); the rest of the buffer is scratch.  A caller that only wants log-probs (the

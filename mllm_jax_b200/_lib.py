@@ -29,7 +29,7 @@ EXPORTS = (
     "mllm_grpo_preference_logps", "mllm_grpo_preference_workspace_bytes",
     "mllm_grpo_embedding_lookup", "mllm_grpo_embedding_grad", "mllm_grpo_embedding_workspace_bytes",
     "mllm_lm_head_fp8_quantize", "mllm_lm_head_fp8_matmul", "mllm_lm_head_fp8_partials",
-    "mllm_lm_head_fp8_partials_bytes",
+    "mllm_lm_head_fp8_partials_bytes", "mllm_lm_head_fp8_stop_after",
 )
 
 
@@ -192,6 +192,8 @@ def load():
         fn = getattr(lib, name)
         fn.argtypes = [C.c_int64, C.c_int64]
         fn.restype = C.c_int64
+    lib.mllm_lm_head_fp8_stop_after.argtypes = [C.c_int32]
+    lib.mllm_lm_head_fp8_stop_after.restype = None
     lib.mllm_ppo_value_workspace_bytes.argtypes = [C.c_int64, C.c_int64]
     lib.mllm_ppo_value_workspace_bytes.restype = C.c_int64
     lib.mllm_grpo_workspace_bytes.argtypes = [C.c_int64]

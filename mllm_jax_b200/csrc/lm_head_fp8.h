@@ -11,6 +11,7 @@ struct Params {
   int64_t n_rows, vocab, hidden, hidden_stride, weight_stride, out_stride, vocab_start, vocab_total;
   int m_tiles, n_tiles, k_blocks, tiles_per_split, splits;
   int out_aligned;  // rows of out start on 16-byte boundaries
+  int stop_after;   // tiles of a CTA (pair) that are multiplied: all, unless a test makes the waits run out
   float softcap;
   const uint8_t* x;
   const uint8_t* w;

@@ -29,6 +29,12 @@
 //
 // The finished tile goes through shared memory and leaves by TMA while the next one is accumulated (threads writing
 // their own rows: 4096 cycles per tile; coalesced stores from shared memory: 3300).
+//
+// Every wait is bounded.  When one runs out, the epilogue writes NaN to the elements of its tiles that it has not
+// reached, so that a product nobody checked the status of cannot be taken for one.
+#include <atomic>
+#include <type_traits>
+
 #include "grpo_launch.h"
 #include "grpo_tc.cuh"
 #include "lm_head_fp8.h"
@@ -319,6 +325,16 @@ __device__ __forceinline__ void store_rows(const Params& p, const CUtensorMap* m
   }
 }
 
+// NaN in a warp's 32 rows x valid columns of a tile that will not be computed.
+template <typename O>
+__device__ __forceinline__ void void_rows(const Params& p, int64_t row0, int64_t n0, int valid, int lane) {
+  using Bits = typename std::conditional<sizeof(O) == 4, uint32_t, uint16_t>::type;
+  for (int64_t row = row0; row < row0 + 32 && row < p.n_rows; ++row) {
+    Bits* const to = static_cast<Bits*>(p.out) + row * p.out_stride + n0;
+    for (int c = lane; c < valid; c += 32) to[c] = Bits(~Bits(0)) >> 1;
+  }
+}
+
 // STATS: fold the tiles into (max, sumexp, sum e*y, chosen) instead of writing them as O.
 template <int BN, int CTAS, bool STATS, typename O>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -436,7 +452,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
       bool ok = true;
-      for (int t = 0; t < n_mine && ok; ++t) {
+      const int n_tiles = min(n_mine, p.stop_after);
+      for (int t = 0; t < n_tiles && ok; ++t) {
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           // the tiles are there long before the accumulator is free: that wait comes last, with everything prepared
           ok = wait_or_abort(full_bar(stage), phase, &abort_flag, p.device_status);
@@ -536,7 +553,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       c -= p.vocab_start;
       if (c < 0 || c >= p.vocab) c = -1;
     }
-    for (int t = 0; t < n_mine && ok; ++t) {
+    int t = 0;
+    for (; t < n_mine; ++t) {
       int m_tile, n_tile;
       tile_at(t, &m_tile, &n_tile);
       const int64_t n0 = int64_t(n_tile) * BN + half * CW;
@@ -632,8 +650,14 @@ product_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       if (row < p.n_rows)
         p.partials[(int64_t(split) * 2 + half + 1) * p.n_rows + row] =
             ok ? make_float4(m, s, u, yc) : make_float4(kNegInit, 0.f, 0.f, 0.f);
-    } else if (lane == 0) {
-      cl::bulk_wait_all();  // the buffers are read and written out before this CTA's shared memory goes
+    } else {
+      for (; t < n_mine; ++t) {  // a wait has run out in tile t
+        int m_tile, n_tile;
+        tile_at(t, &m_tile, &n_tile);
+        const int64_t n0 = int64_t(n_tile) * BN + half * CW;
+        void_rows<O>(p, int64_t(m_tile) * kBM + quarter * 32, n0, int(p.vocab - n0 < CW ? p.vocab - n0 : CW), lane);
+      }
+      if (lane == 0) cl::bulk_wait_all();  // the buffers are read and written out before this CTA's shared memory goes
     }
   }
 
@@ -800,6 +824,8 @@ static int launch_product(const Params& p, const mllm_lm_head_fp8_args* a, cudaS
   return ctas_for(m_tiles) == 2 ? launch<256, 2, false, O>(p, a, s) : launch<256, 1, false, O>(p, a, s);
 }
 
+static std::atomic<int> stop_after{-1};  // test hook
+
 static bool aligned(const void* q, uintptr_t a) { return (reinterpret_cast<uintptr_t>(q) & (a - 1)) == 0; }
 
 static int check(const mllm_lm_head_fp8_args* a, Params* p) {
@@ -833,6 +859,8 @@ static int check(const mllm_lm_head_fp8_args* a, Params* p) {
   p->partials = static_cast<float4*>(a->partials);
   p->softcap = a->softcap;
   p->device_status = a->device_status;
+  const int stop = stop_after.load(std::memory_order_relaxed);
+  p->stop_after = stop < 0 ? INT32_MAX : stop;
   return MLLM_GRPO_OK;
 }
 
@@ -842,6 +870,8 @@ static int check(const mllm_lm_head_fp8_args* a, Params* p) {
 using namespace grpo;
 
 extern "C" {
+
+void mllm_lm_head_fp8_stop_after(int32_t tiles) { fp8::stop_after.store(tiles, std::memory_order_relaxed); }
 
 int mllm_lm_head_fp8_matmul(const mllm_lm_head_fp8_args* a, void* stream) {
   fp8::Params p;

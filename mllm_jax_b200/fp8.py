@@ -131,8 +131,9 @@ def fp8_matmul(x: Union[Fp8Blocks, torch.Tensor], w: Fp8Blocks, *, out_dtype: to
                out: Optional[torch.Tensor] = None, device_status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [M, K] (Fp8Blocks with blocks of (1, 128), or a tensor, which is quantised first) times w [N, K] (blocks of
     (128, 128)), transposed: [M, N] of out_dtype (bf16, f16 or f32), rounded once.  K must be a multiple of 16.
-    `out` [M, N] (rows any distance apart) is written instead of a new tensor when given.  device_status (an int32 CUDA
-    tensor of the caller) has MLLM_GRPO_DEV_WAIT_TIMEOUT set if a wait inside the kernel ran out: the product is void."""
+    `out` [M, N] (rows any distance apart) is written instead of a new tensor when given.  If a wait inside the kernel runs
+    out, the elements that were not reached are NaN and device_status (an int32 CUDA tensor of the caller), where one is
+    passed, has MLLM_GRPO_DEV_WAIT_TIMEOUT set."""
     if not isinstance(x, Fp8Blocks):
         x = quantize_fp8(x, block=(1, BLOCK))
     a = _bind(x, w)

@@ -466,3 +466,32 @@ def test_folded_head_over_a_process_group_of_one(cuda, tmp_path):
         dist.destroy_process_group()
     for k in ("per_token_logps", "token_entropy", "lse"):
         assert torch.equal(out[k], want[k])
+
+
+# rows, columns, output tiles multiplied by a CTA (pair) before it stops, whether some of the product is there
+@pytest.mark.parametrize("M,N,tiles,some", [(40, 700, 0, False), (300, 515, 0, False), (260, 33001, 1, True), (2049, 33000, 0, False)])
+@pytest.mark.parametrize("out_dtype", TYPES)
+def test_what_a_run_out_wait_leaves_is_nan(cuda, out_dtype, M, N, tiles, some):
+    """A wait that runs out makes every element that was not reached a NaN, with a status word or without one, and
+    nothing outside of out is written; the next call is as ever."""
+    if M * N > 10 ** 6 and out_dtype != torch.bfloat16:
+        return
+    from mllm_jax_b200 import _lib
+    lib = _lib.load()
+    x, w = _operands(M, N, 272, 120, cuda)
+    want = G.fp8_matmul(x, w, out_dtype=out_dtype)
+    stride = N + 3
+    buf = torch.full((M * stride + 16,), 3.0, dtype=out_dtype, device=cuda)
+    out = buf[8:8 + M * stride].view(M, stride)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    lib.mllm_lm_head_fp8_stop_after(tiles)
+    try:
+        G.fp8_matmul(x, w, out=out[:, :N], device_status=status if M != 40 else None)
+        torch.cuda.synchronize()
+    finally:
+        lib.mllm_lm_head_fp8_stop_after(-1)
+    assert M == 40 or int(status) == _lib.DEV_WAIT_TIMEOUT
+    void = torch.isnan(out[:, :N])
+    assert torch.equal(torch.where(void, want, out[:, :N]), want) and bool(void.any()) and bool((~void).any()) == some
+    assert bool((out[:, N:] == 3).all()) and bool((buf[:8] == 3).all()) and bool((buf[8 + M * stride:] == 3).all())
+    assert torch.equal(G.fp8_matmul(x, w, out_dtype=out_dtype), want)
