@@ -162,6 +162,8 @@ def _fp8_logprobs(a, hq: torch.Tensor, place: int, weight: Fp8Blocks, token_ids,
     lp, ent, lse = out.unbind(0)
     a.chosen_ids, a.partials, a.call_status = ids.data_ptr(), workspace.data_ptr(), hq.data_ptr() + place
     a.softcap, a.temperature = float(cfg.softcap) if cfg.softcap else 0.0, cfg.temperature
+    if not a.temperature > 0:  # the struct's 0 stands for 1
+        raise ValueError(f"temperature must be positive, got {cfg.temperature}")
     a.per_token_logps, a.lse = lp.data_ptr(), lse.data_ptr()
     if cfg.compute_entropy:
         a.token_entropy = ent.data_ptr()

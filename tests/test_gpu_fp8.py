@@ -495,3 +495,16 @@ def test_what_a_run_out_wait_leaves_is_nan(cuda, out_dtype, M, N, tiles, some):
     assert torch.equal(torch.where(void, want, out[:, :N]), want) and bool(void.any()) and bool((~void).any()) == some
     assert bool((out[:, N:] == 3).all()) and bool((buf[:8] == 3).all()) and bool((buf[8 + M * stride:] == 3).all())
     assert torch.equal(G.fp8_matmul(x, w, out_dtype=out_dtype), want)
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1e-60, -1.0, float("nan")])
+def test_a_temperature_that_is_not_positive_is_refused(cuda, temperature):
+    """By heads of both kinds, with and without the loss (1e-60 is 0 in the 32 bits that the kernels take)."""
+    B, T, H, V = 1, 4, 64, 256
+    hidden, plain = _x(T, H, torch.bfloat16, 114, cuda).view(B, T, H), _x(V, H, torch.bfloat16, 115, cuda)
+    ids = torch.zeros(B, T, dtype=torch.int32, device=cuda)
+    cfg = G.LossConfig(temperature=temperature, compute_entropy=False)
+    for weight in (plain, G.quantize_fp8(plain, block=(128, 128))):
+        for adv in (None, torch.ones(B, device=cuda)):
+            with pytest.raises((ValueError, G.GrpoError)):
+                lm_head_forward(hidden, weight, ids, advantages=adv, cfg=cfg)
