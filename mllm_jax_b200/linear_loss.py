@@ -27,6 +27,13 @@ from .fp8 import Fp8Blocks, _quantize_and_bind
 from .ops import LossConfig, TokenLossProblem
 
 
+def _workspace_bytes(t: torch.Tensor, nbytes: int, dev: torch.device) -> torch.Tensor:
+    """A caller's workspace, of any type, as the bytes that a call of `nbytes` on `dev` writes."""
+    if t.device != dev or not t.is_contiguous() or t.numel() * t.element_size() < nbytes or t.data_ptr() % 16:
+        raise ValueError(f"workspace must hold {nbytes} contiguous bytes at a 16-byte aligned address on {dev}")
+    return t if t.dtype is torch.uint8 and t.dim() == 1 else t.view(-1).view(torch.uint8)
+
+
 def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks], token_ids: torch.Tensor,
                     mask: Optional[torch.Tensor] = None, advantages: Optional[torch.Tensor] = None,
                     total_valid_token_count=None, old_per_token_logps: Optional[torch.Tensor] = None,
@@ -47,7 +54,8 @@ def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]
     (the reference-model pass, train_modules/__init__.py:129-132, and plugins/training/update/ppo.py:39-43).
     Two launches: the tensor-core kernel writes per-row partials for each vocabulary range, and
     mllm_grpo_combine merges them and runs the per-token epilogue.  H must be a multiple of 64.
-    The logits are the f32 accumulators (not rounded to bf16 on the way).
+    The logits are the f32 accumulators (not rounded to bf16 on the way).  workspace: a contiguous tensor of any type on
+    hidden's device that holds mllm_lm_head_partials_bytes (8-bit head: mllm_lm_head_fp8_partials_bytes), for this call.
 
     weight may be `Fp8Blocks` [V, H] with blocks of (128, 128) (`quantize_fp8(weight, block=(128, 128))`): hidden is
     quantised with a scale per 1 x 128 on the way in and both run as 8-bit operands (mllm_lm_head_fp8_partials; H a
@@ -93,8 +101,8 @@ def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]
         nbytes = int(lib.mllm_lm_head_partials_bytes(N, V))
     if workspace is None:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    elif workspace.numel() * workspace.element_size() < nbytes or workspace.data_ptr() % 16:
-        raise ValueError(f"workspace must hold {nbytes} bytes at a 16-byte aligned address")
+    else:
+        workspace = _workspace_bytes(workspace, nbytes, dev)
     forward_only = advantages is None
     if fp8 and forward_only and group is None and vocab_start == 0 and vocab_total in (None, V) and \
             total_valid_token_count is None and old_per_token_logps is None and ref_per_token_logps is None:

@@ -508,3 +508,27 @@ def test_a_temperature_that_is_not_positive_is_refused(cuda, temperature):
         for adv in (None, torch.ones(B, device=cuda)):
             with pytest.raises((ValueError, G.GrpoError)):
                 lm_head_forward(hidden, weight, ids, advantages=adv, cfg=cfg)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+def test_workspaces_of_any_type(cuda, monkeypatch, kind):
+    """A workspace of floats serves as one of bytes, alone and where a part of it is gathered; one of the host is refused."""
+    from mllm_jax_b200 import _lib
+    B, T, H, V = 1, 10, 64, 512
+    hidden, plain = _x(T, H, torch.bfloat16, 130, cuda).view(B, T, H), _x(V, H, torch.bfloat16, 131, cuda)
+    weight = plain if kind == "bf16" else G.quantize_fp8(plain, block=(128, 128))
+    ids = torch.randint(0, V, (B, T), generator=torch.Generator().manual_seed(132)).to(cuda)
+    lib = _lib.load()
+    nbytes = (lib.mllm_lm_head_partials_bytes if kind == "bf16" else lib.mllm_lm_head_fp8_partials_bytes)(T, V)
+    room = torch.empty(nbytes // 4, device=cuda)
+    sent = []
+    _gathered(monkeypatch, 1, sent)
+    adv = torch.zeros(B, device=cuda)
+    want = lm_head_forward(hidden, weight, ids, advantages=adv)
+    for extra in ({}, dict(group=object())):
+        out = lm_head_forward(hidden, weight, ids, advantages=adv, workspace=room, **extra)
+        for k in ("per_token_logps", "token_entropy", "lse"):
+            assert torch.equal(out[k], want[k])
+    assert sent[0].dtype == torch.uint8
+    with pytest.raises(ValueError, match="workspace"):
+        lm_head_forward(hidden, weight, ids, workspace=torch.empty(nbytes, dtype=torch.uint8))

@@ -252,3 +252,18 @@ def test_forward_mode_tangents_are_refused():
         _lib.no_tangent(t, "t")
         with pytest.raises(NotImplementedError, match="t carries a forward-mode tangent"):
             _lib.no_tangent(fwd.make_dual(t, torch.ones(3)), "t")
+
+
+def test_a_workspace_is_checked_before_a_kernel_writes_it():
+    """Its device (an address of the host's memory would be written by the kernel), its layout, its size in bytes; of any
+    type it is taken as bytes, which a gather over ranks counts."""
+    from mllm_jax_b200.linear_loss import _workspace_bytes
+
+    cpu, room = torch.device("cpu"), torch.zeros(64, dtype=torch.float32)
+    got = _workspace_bytes(room, 256, cpu)
+    assert got.dtype == torch.uint8 and got.shape == (256,) and got.data_ptr() == room.data_ptr()
+    assert _workspace_bytes(room.view(8, 8), 200, cpu)[:16].numel() == 16
+    for bad, nbytes, dev in ((room, 257, cpu), (room, 16, torch.device("cuda:0")), (room.view(8, 8)[:, :4], 16, cpu),
+                             (room[1:], 16, cpu)):
+        with pytest.raises(ValueError, match="workspace"):
+            _workspace_bytes(bad, nbytes, dev)
