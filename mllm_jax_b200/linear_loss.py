@@ -80,6 +80,8 @@ def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]
     if fp8:
         if weight.shape[1] != H:
             raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not match")
+        if token_ids.dtype is torch.int64:
+            token_ids = token_ids.clamp(-1, 2 ** 31 - 1)  # an id beyond 32 bits must not wrap to a valid one
     elif weight.shape[0 if hv else 1] != H or hidden.stride(2) != 1 or weight.stride(1) != 1 or \
             hidden.stride(0) != T * hidden.stride(1):
         raise ValueError(f"hidden {tuple(hidden.shape)} / weight {tuple(weight.shape)}: need [B, T, H] rows evenly "
@@ -163,8 +165,6 @@ def _fp8_logprobs(a, hq: torch.Tensor, place: int, weight: Fp8Blocks, token_ids,
     vocabulary ranges and writes the results."""
     if token_ids.numel() != B * T:
         raise ValueError(f"chosen ids must have {B}x{T} elements, got shape {tuple(token_ids.shape)}")
-    if token_ids.dtype is torch.int64:
-        token_ids = token_ids.clamp(-1, 2 ** 31 - 1)  # an id beyond 32 bits must not wrap to a valid one
     ids = token_ids.to(device=dev, dtype=torch.int32).contiguous()
     out = torch.empty(3, B, T, dtype=torch.float32, device=dev)
     lp, ent, lse = out.unbind(0)

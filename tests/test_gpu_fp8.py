@@ -532,3 +532,16 @@ def test_workspaces_of_any_type(cuda, monkeypatch, kind):
     assert sent[0].dtype == torch.uint8
     with pytest.raises(ValueError, match="workspace"):
         lm_head_forward(hidden, weight, ids, workspace=torch.empty(nbytes, dtype=torch.uint8))
+
+
+def test_folded_head_with_a_loss_clamps_ids_beyond_32_bits(cuda):
+    """As without one: such an id is the vocabulary's end and is reported, not the id that its lower 32 bits spell."""
+    B, T, H, V = 1, 6, 64, 300
+    hidden = _x(T, H, torch.bfloat16, 96, cuda).view(B, T, H)
+    w = G.quantize_fp8(_x(V, H, torch.bfloat16, 97, cuda), block=(128, 128))
+    ids = torch.tensor([[0, 5, 2 ** 32 + 5, -(2 ** 32) + 5, V, V - 1]], device=cuda)
+    near = torch.tensor([[0, 5, V - 1, 0, V - 1, V - 1]], device=cuda)
+    adv = torch.ones(B, device=cuda)
+    out, want = (lm_head_forward(hidden, w, i, advantages=adv) for i in (ids, near))
+    assert torch.equal(out["per_token_logps"], want["per_token_logps"])
+    assert G.ops.check_device_status(out["problem"]) == 1 and G.ops.check_device_status(want["problem"]) == 0
