@@ -70,6 +70,8 @@ def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]
         raise RuntimeError("lm_head_forward needs CUDA tensors: the kernels have no CPU path")
     if hidden.dtype != torch.bfloat16 or (not fp8 and weight.dtype != torch.bfloat16):
         raise TypeError("hidden and weight must be bfloat16")
+    if weight.device != hidden.device:
+        raise ValueError(f"hidden is on {hidden.device} and weight on {weight.device}")
     B, T, H = hidden.shape
     if fp8 and weight_layout != "vh":
         raise ValueError("an 8-bit weight is [V, H]")

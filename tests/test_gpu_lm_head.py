@@ -181,3 +181,15 @@ def test_folded_forward_on_a_vocabulary_shard(cuda):
     assert (prob.per_token_logps.cpu().double() - ref["per_token_logps"]).abs().max() <= LP_ATOL
     assert (prob.token_entropy.cpu().double() - ref["token_entropy"]).abs().max() <= ENT_ATOL
     assert_loss_close(prob.loss.item(), ref["loss"].item())
+
+
+def test_a_weight_of_another_device_is_refused(cuda):
+    """Its address would be read by the kernel."""
+    from mllm_jax_b200.fp8 import Fp8Blocks
+    hidden = torch.zeros(1, 4, 128, dtype=torch.bfloat16, device=cuda)
+    ids = torch.zeros(1, 4, dtype=torch.int32, device=cuda)
+    values = torch.zeros(256, 128, dtype=torch.float8_e4m3fn)
+    for weight, kw in ((torch.zeros(256, 128, dtype=torch.bfloat16), {}), (Fp8Blocks(values, torch.ones(2, 1)), {}),
+                       (torch.zeros(128, 256, dtype=torch.bfloat16), dict(weight_layout="hv"))):
+        with pytest.raises(ValueError, match="weight on cpu"):
+            lm_head_forward(hidden, weight, ids, **kw)
