@@ -426,7 +426,8 @@ int64_t mllm_grpo_embedding_workspace_bytes(int64_t n_tokens, int64_t hidden, in
 
 /* ---- 8-bit floating point (e4m3) with a scale for each block of 128 ----
  * scale = max(amax, 448 * 2^-126) / 448 over a block of block_rows x 128 elements, q = e4m3(448 x / amax) to nearest
- * even; blocks at the right and lower edge are shorter.  A NaN stays a NaN and is left out of the maximum; an
+ * even (of f32 inputs a quotient within 2^-19, relative, of the middle between two values counts as the middle; 16-bit
+ * inputs are rounded exactly); blocks at the right and lower edge are shorter.  A NaN stays a NaN and is left out of the maximum; an
  * infinity makes its block's scale infinite. */
 typedef struct mllm_lm_head_fp8_quantize_args {
   uint64_t struct_size;

@@ -28,7 +28,7 @@ struct Params {
 };
 
 // The product for at most kFewRows rows of x (lm_head_fp8_rows.cu).  One tile of 8 tokens: 151936 x 3584 in 90 us for
-// any of them (tensor-memory tiles: 105-113 us); a second tile of 8 took 126 us, more than the tiles do.
+// any of them (tensor-memory tiles: 105-131 us for 9 to 128 rows, from run to run); a second tile of 8 took 126 us, no less.
 constexpr int64_t kFewRows = 8;
 cudaError_t launch_few_rows(const Params& p, int out_dtype, cudaStream_t s);
 

@@ -56,7 +56,8 @@ class Fp8Blocks:
 
 def quantize_fp8(x: torch.Tensor, *, block: Tuple[int, int] = (1, BLOCK)) -> Fp8Blocks:
     """x [R, C] bf16 / f16 / f32 (rows any distance apart) -> Fp8Blocks with q = e4m3(448 x / amax of the block), to
-    nearest even, and scale = amax / 448 (at least 2^-126).  Blocks at the edges are shorter."""
+    nearest even, and scale = amax / 448 (at least 2^-126).  Blocks at the edges are shorter.  16-bit inputs are rounded
+    exactly so; of f32 inputs a quotient within 2^-19 (relative) of the middle between two values counts as the middle."""
     if not x.is_cuda:
         raise RuntimeError("quantize_fp8 needs CUDA tensors: the kernels have no CPU path")
     if x.dtype not in _DTYPES:

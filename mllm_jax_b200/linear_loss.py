@@ -60,7 +60,9 @@ def lm_head_forward(hidden: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]
     weight may be `Fp8Blocks` [V, H] with blocks of (128, 128) (`quantize_fp8(weight, block=(128, 128))`): hidden is
     quantised with a scale per 1 x 128 on the way in and both run as 8-bit operands (mllm_lm_head_fp8_partials; H a
     multiple of 16, any distance between the rows of hidden).  The head of a frozen reference model takes half the
-    memory that way; the log-probs are those of the quantised operands."""
+    memory that way; the log-probs are those of the quantised operands.  Without a loss (no advantages, counts or other
+    log-probs) and without shards, the returned `problem` holds the call's device_status only, and the entropy is formed
+    whether cfg.compute_entropy asks for it or not."""
     cfg = cfg or LossConfig()
     fp8 = isinstance(weight, Fp8Blocks)
     if hidden.dim() == 2:
